@@ -386,6 +386,73 @@ int b200_qk_norm_rope_kv_write(
     int num_blocks, int max_pages, int max_requests, int layer,
     int32_t* dev_status, void* stream);
 
+/*
+ * RMS norm with the residual's addition, in bf16 or in 8 bits (no counterpart
+ * in the reference, whose norm and residual are separate torch operations,
+ * qwen3/norm.py:22-26).  For each of `rows` rows of `hidden` elements:
+ *     h = x + residual (fp32)      residual_out = bf16(h)
+ *     y = h / sqrt(mean(h^2) + eps) * weight
+ * scale == NULL: y as bf16.  scale != NULL: scale[row] = max(max|y|, 1e-12) / 448
+ * and y holds e4m3(y / scale[row]).  residual and residual_out come together
+ * or not at all.  weight == NULL: no norm, y = x (needs scale, no residual).
+ * Row strides in elements; rows contiguous; x, residual, weight, residual_out
+ * bf16.  residual_out may be residual or x.  Rows that are 16-byte aligned
+ * take the vector path, others any alignment.
+ */
+int b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                  const void* weight, void* y, int64_t y_stride, float* scale,
+                  void* residual_out, int64_t h_stride, int64_t rows, int hidden, float eps,
+                  void* stream);
+
+/* Activations of b200_linear. */
+#define B200_ACT_NONE 0
+#define B200_ACT_RELU 1
+#define B200_ACT_SILU 2
+#define B200_ACT_GELU 3      /* with the error function */
+#define B200_ACT_GELU_TANH 4 /* with the tanh approximation */
+
+/*
+ * Matrix product with bias, activation and residual in its epilogue:
+ *   out = act(s (x w^T) + bias) + residual                          gated == 0
+ *   out = act(gate) * up + residual, w = [n gate rows; n up rows]   gated == 1
+ * x (m, k), w (n or 2n, k): bf16, or e4m3 with fp8 != 0 and then x_scale (m,)
+ * and w_scale (n or 2n,) fp32, s = x_scale[t] * w_scale[row].  bias (n or 2n,),
+ * residual (m, n), out (m, n) bf16; x_scale, w_scale, bias and residual are
+ * NULL where unused.  Row strides in elements, rows contiguous; x and w start on
+ * 16 bytes and their row strides are multiples of 16 bytes (k itself need not
+ * be); out may be residual.  Sums in fp32, one rounding.
+ */
+int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+                int64_t w_stride, const float* w_scale, const void* bias, const void* residual,
+                int64_t r_stride, void* out, int64_t o_stride, int m, int n, int k, int fp8,
+                int gated, int activation, int32_t* dev_status, void* stream);
+
+/*
+ * Rotary positions of q (batch, num_heads, seq, head_dim) and k (batch,
+ * num_kv_heads, seq, head_dim), bf16 with strides (batch, head, token); q_out
+ * and k_out may be q and k.  Of every head the first rotary_dim elements turn
+ * (pairs i, i + rotary_dim / 2, or 2i, 2i + 1 when interleaved), the rest is
+ * copied.  turns: rotary_dim / 2 fractions of a turn a position, in units of
+ * 2^-64; gain multiplies cos and sin.  positions: int32 or int64 (batch, seq)
+ * with strides.  num_heads or num_kv_heads may be 0.
+ * (The reference turns by tables, qwen3/rope.py:88-110.)
+ */
+int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                const void* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                void* q_out, int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_s,
+                void* k_out, int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_s,
+                const void* positions, int64_t pos_stride_b, int64_t pos_stride_s,
+                int positions_64, const uint64_t* turns, float gain, int batch, int seq,
+                int num_heads, int num_kv_heads, int head_dim, int rotary_dim, int interleaved,
+                void* stream);
+
+/* cos and sin rows (batch, seq, rotary_dim) fp32, contiguous, of the same plan:
+ * what b200_qk_norm_rope_kv_write takes (half layout). */
+int b200_rotary_tables(const void* positions, int64_t pos_stride_b, int64_t pos_stride_s,
+                       int positions_64, const uint64_t* turns, float gain, float* cos_out,
+                       float* sin_out, int batch, int seq, int rotary_dim, int interleaved,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,10 @@ Hand-written CUDA kernels behind the C ABI in ``include/qwen3_b200_attn.h``:
 * varlen causal prefill attention (tcgen05 MMAs with TMEM accumulators, TMA
   tiles, persistent CTAs), also over the paged cache (chunked prefill);
 * KV-cache slot scatter (row-addressed and slot_mapping-addressed);
-* the fused QK-RMSNorm + RoPE + KV write prologue and the fused token sampler.
+* the fused QK-RMSNorm + RoPE + KV write prologue and the fused token sampler;
+* the rest of the decoder layer: RMS norm with the residual's addition and an
+  8-bit output, matrix products with a fused epilogue (tcgen05, bf16 and e4m3),
+  rotary positions with frequencies scaled for long contexts (``rope``).
 
 ``ops`` holds the reference-facing functions (same names and arguments as the
 reference engine's kernel wrappers), ``paged_kv`` the host-side pool / request
@@ -36,8 +39,15 @@ from .ops import (  # noqa: F401
     clear_device_status,
     check_device_status,
     decode_workspace_bytes,
+    rms_norm,
+    rms_norm_fp8,
+    quantize_rows_fp8,
+    linear,
+    rotary,
+    rotary_tables,
 )
 from .paged_kv import KVCachePool, PagedKVCache  # noqa: F401
+from .rope import RotaryPlan, rotary_frequencies  # noqa: F401
 from .graph_runner import GraphRunner, kv_pool_blocks  # noqa: F401
 
 __version__ = "0.1.0"

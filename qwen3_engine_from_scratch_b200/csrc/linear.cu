@@ -1,0 +1,600 @@
+// Matrix product with a fused epilogue, for sm_100a's tcgen05 tensor cores:
+//   out = act(sx_t sw_n (X W^T)_tn + b_n) + r_tn                    plain
+//   out = act(gate_tn) up_tn + r_tn, W = [gate rows; up rows]       gated
+// X (m, k) and W (n or 2n, k) in bf16, or in e4m3 with an fp32 scale a row of
+// each; accumulators, scales, bias, activation and residual in fp32, one
+// rounding to bf16 at the end.
+//
+// The weight's rows are the M side of the instruction (128 TMEM lanes) and the
+// tokens its N side: a decode step of a few tokens then streams W through full
+// 128-row tiles and pads only the small token side, and one kernel serves one
+// token and thousands.  Token tiles of BN columns; two accumulators of BN
+// columns, so the epilogue of one tile overlaps the product of the next.
+//   warps 0-3  epilogue: lane l of warp w owns accumulator lane 32 w + l
+//   warp 4     TMA producer (one lane): 128-byte swizzled K-major tiles,
+//              128 weight rows and BN tokens x 128 bytes of K a stage
+//   warp 5     MMA issuer (one lane): 4 instructions a stage (K = 32 bytes)
+// Gated: lanes 0-15 of every warp hold gate rows and lanes 16-31 the up rows
+// of the same 16 outputs, so the two meet by one shuffle; the tile's rows
+// come from one 4-D box (k, 16, gate/up, group) where n is a multiple of 16, or
+// from 8 boxes of 16 rows.  Neighbouring lanes exchange values of neighbouring
+// tokens before the store, so a lane writes two outputs (4 bytes) of one token
+// and a warp whole 32-byte sectors.
+//
+// Few tiles (a decode step): the CTAs of a cluster share one tile and split K;
+// every CTA sends its fp32 partial to the CTA that owns its token columns
+// through distributed shared memory, and the owners add the partials in rank
+// order, so the result does not depend on timing.
+//
+// Every wait is bounded: one that runs out sets B200_DEV_TIMEOUT, the other
+// roles give up too, outstanding copies are awaited and TMEM is freed.
+#include <mutex>
+
+#include "tcgen05.cuh"
+
+namespace {
+
+using namespace b200;
+
+constexpr int kRows = 128;        // weight rows of a tile (TMEM lanes)
+constexpr int kKBytes = 128;      // bytes of K a stage: one swizzle row
+constexpr int kABytes = kRows * kKBytes;
+constexpr int kThreads = 192;
+constexpr int kEpilogueThreads = 128;
+constexpr int kProducerWarp = 4;
+constexpr int kMmaWarp = 5;
+constexpr int kMaxStages = 10;
+constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
+constexpr int kMaxSplits = 8;
+constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
+constexpr uint64_t kWaitLimitNs = 1000000000ull;
+
+struct LinearArgs {
+  const float* x_scale;  // nullable together
+  const float* w_scale;
+  const __nv_bfloat16* bias;      // nullable
+  const __nv_bfloat16* residual;  // nullable
+  __nv_bfloat16* out;
+  int64_t r_row, o_row;
+  int m, n;
+  int k_blocks;          // blocks of 128 bytes of K
+  int m_tiles, n_tiles;
+  int gated;             // 0, 1: boxes of 16 rows, 2: one 4-D box
+  int act;
+  int splits;            // CTAs of a cluster, each with a share of K
+  int stages;
+  int pairs;             // out and residual take 4-byte accesses
+  int32_t* dev_status;
+};
+
+struct __align__(8) Barriers {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int32_t error;
+};
+
+B200_DEVICE bool wait_or_flag(uint32_t bar, uint32_t parity, Barriers* B, int32_t* dev_status) {
+  if (mbar_wait_abortable(bar, parity, dev_status, kWaitLimitNs)) return true;
+  if (atomicExch(&B->error, 1) == 0) flag_error(dev_status, B200_DEV_TIMEOUT);
+  return false;
+}
+
+// c format f32, a / b format bf16 (1) of kind::f16 or e4m3 (0) of kind::f8f6f4, both K-major
+template <bool FP8>
+constexpr uint32_t instruction(uint32_t n) {
+  return (1u << 4) | ((FP8 ? 0u : 1u) << 7) | ((FP8 ? 0u : 1u) << 10) | ((n >> 3) << 17) |
+         ((static_cast<uint32_t>(kRows) >> 4) << 24);
+}
+
+template <bool FP8>
+B200_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (FP8) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+B200_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+B200_DEVICE uint32_t remote_smem(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+B200_DEVICE void st_remote(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+B200_DEVICE float ld_shared(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+B200_DEVICE float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+
+B200_DEVICE float activate(float v, int act) {
+  switch (act) {
+    case B200_ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN stays
+    case B200_ACT_SILU: return v * sigmoid(v);
+    case B200_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    case B200_ACT_GELU_TANH:  // (1 + tanh z) / 2 = sigmoid(2 z)
+      return v * sigmoid(1.5957691216057308f * (v + 0.044715f * v * v * v));
+    default: return v;
+  }
+}
+
+struct Tile {
+  int token0, n0;
+};
+
+// Tiles in groups of kGroupTokens token tiles: within a group the token tiles
+// of one weight tile come one after another, so the CTAs at work at a time
+// share few weight tiles and few token tiles in L2.
+template <int BN>
+B200_DEVICE Tile tile_at(const LinearArgs& a, int tile) {
+  const int per_group = kGroupTokens * a.n_tiles;
+  const int g = tile / per_group;
+  const int first = g * kGroupTokens;
+  const int rows = min(kGroupTokens, a.m_tiles - first);
+  const int rem = tile - g * per_group;
+  Tile t;
+  t.token0 = (first + rem % rows) * BN;
+  t.n0 = rem / rows * (a.gated ? kRows / 2 : kRows);
+  return t;
+}
+
+// A lane's share of the epilogue of a tile: turns raw accumulators of this
+// lane's row into outputs.
+struct Epilogue {
+  const LinearArgs& a;
+  int lane, row_n;   // output column of this lane
+  int pair_n;        // first of the two output columns this lane writes
+  float w_scale, bias;
+
+  B200_DEVICE Epilogue(const LinearArgs& args, int n0, int warp, int l) : a(args), lane(l) {
+    row_n = a.gated ? n0 + warp * 16 + (l & 15) : n0 + warp * 32 + l;
+    pair_n = row_n & ~1;
+    const int w_row = a.gated && l >= 16 ? a.n + row_n : row_n;
+    const bool live = row_n < a.n;
+    w_scale = a.w_scale != nullptr && live ? a.w_scale[w_row] : 1.0f;
+    bias = a.bias != nullptr && live ? __bfloat162float(a.bias[w_row]) : 0.0f;
+  }
+
+  // outputs (token, pair_n) and (token, pair_n + 1)
+  B200_DEVICE void put(int token, float lo, float hi) const {
+    if (token >= a.m || pair_n >= a.n) return;
+    __nv_bfloat16* o = a.out + token * a.o_row + pair_n;
+    const __nv_bfloat16* r =
+        a.residual != nullptr ? a.residual + token * a.r_row + pair_n : nullptr;
+    if (a.pairs) {
+      if (r != nullptr) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(r);
+        lo += bf16_lo(w);
+        hi += bf16_hi(w);
+      }
+      *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(lo, hi);
+    } else {
+      if (r != nullptr) lo += __bfloat162float(r[0]);
+      o[0] = __float2bfloat16_rn(lo);
+      if (pair_n + 1 < a.n) {
+        if (r != nullptr) hi += __bfloat162float(r[1]);
+        o[1] = __float2bfloat16_rn(hi);
+      }
+    }
+  }
+
+  // this lane's v0 of `token` and v1 of `token + step`: the even lane of a
+  // pair writes the first token's two outputs, the odd lane the second's
+  B200_DEVICE void put_pair(int token, int step, float v0, float v1) const {
+    const bool odd = lane & 1;
+    const float got = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+    put(odd ? token + step : token, odd ? got : v0, odd ? v1 : got);
+  }
+
+  // accumulators of tokens token .. token + 3
+  B200_DEVICE void put4(int token, const float (&acc)[4]) const {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = acc[i];
+      if (a.x_scale != nullptr)
+        v[i] *= w_scale * (token + i < a.m ? __ldg(a.x_scale + token + i) : 0.0f);
+      v[i] += bias;
+    }
+    if (a.gated) {
+      // low half-warp: gate, high half-warp: up; each keeps one token of two
+      const bool high = lane >= 16;
+      float o[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float got = __shfl_xor_sync(0xffffffffu, high ? v[2 * i] : v[2 * i + 1], 16);
+        const float gate = high ? got : v[2 * i];
+        const float up = high ? v[2 * i + 1] : got;
+        o[i] = activate(gate, a.act) * up;
+      }
+      put_pair(token + (high ? 1 : 0), 2, o[0], o[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = activate(v[i], a.act);
+      put_pair(token, 1, v[0], v[1]);
+      put_pair(token + 2, 1, v[2], v[3]);
+    }
+  }
+};
+
+template <int BN, bool FP8>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                  const LinearArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Barriers B;
+  constexpr int kBBytes = BN * kKBytes;
+  constexpr int kStageBytes = kABytes + kBBytes;
+  constexpr int kKElems = FP8 ? 128 : 64;
+  constexpr uint32_t kTmemCols = 2 * BN;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = smem_u32(smem);
+  const uint32_t exchange = base + a.stages * kStageBytes;  // [from rank][column][row] fp32
+  auto full = [&](int s) { return smem_u32(&B.full[s]); };
+  auto empty = [&](int s) { return smem_u32(&B.empty[s]); };
+  auto acc_full = [&](int b) { return smem_u32(&B.acc_full[b]); };
+  auto acc_empty = [&](int b) { return smem_u32(&B.acc_empty[b]); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), kEpilogueThreads);
+    }
+    B.error = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&B.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  if (a.splits > 1) cluster_sync();  // every CTA of the cluster runs before any writes to it
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = B.tmem_base;
+  pdl_begin();
+  // a pipeline already gave up: start no new work until the host clears the status
+  const bool aborted = a.dev_status != nullptr &&
+                       (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
+
+  const int rank = a.splits > 1 ? static_cast<int>(blockIdx.x) % a.splits : 0;
+  const int first = static_cast<int>(blockIdx.x) / a.splits;
+  const int stride = static_cast<int>(gridDim.x) / a.splits;
+  const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / a.splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / a.splits);
+
+  if (warp == kProducerWarp && lane == 0) {
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += stride) {
+      const Tile t = tile_at<BN>(a, tile);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = wait_or_flag(empty(stage), phase ^ 1, &B, a.dev_status))) break;
+        const uint32_t bar = full(stage), dst = base + stage * kStageBytes;
+        const int k0 = kb * kKElems;
+        mbar_arrive_expect_tx(bar, kStageBytes);
+        if (a.gated == 2) {
+          tma_load_4d_nohint(dst, &tm_w, bar, k0, 0, 0, t.n0 / 16);
+        } else if (a.gated == 1) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            tma_load_2d(dst + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
+            tma_load_2d(dst + g * 4096 + 2048, &tm_w, bar, k0, a.n + t.n0 + g * 16);
+          }
+        } else {
+          tma_load_2d(dst, &tm_w, bar, k0, t.n0);
+        }
+        tma_load_2d(dst + kABytes, &tm_x, bar, k0, t.token0);
+        ++issued;
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok) {  // the copies in flight land before the CTA's shared memory goes away
+      for (int i = 0; i < min(issued, a.stages); ++i) {
+        if (--stage < 0) {
+          stage = a.stages - 1;
+          phase ^= 1;
+        }
+        mbar_wait_bounded(full(stage), phase);
+      }
+    }
+  } else if (warp == kMmaWarp && lane == 0) {
+    constexpr uint32_t idesc = instruction<FP8>(BN);
+    int stage = 0, count = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < tiles; tile += stride, ++count) {
+      const int buf = count & 1;
+      if (!(ok = wait_or_flag(acc_empty(buf), ((count >> 1) & 1) ^ 1, &B, a.dev_status))) break;
+      tc_fence_after();
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = wait_or_flag(full(stage), phase, &B, a.dev_status))) break;
+        tc_fence_after();
+        const uint32_t sa = base + stage * kStageBytes, sb = sa + kABytes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma<FP8>(tmem + buf * BN, smem_desc(sa + j * 32, 16, 1024), smem_desc(sb + j * 32, 16, 1024),
+                   idesc, kb > kb0 || j > 0 ? 1u : 0u);
+        umma_commit(empty(stage));
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok) umma_commit(acc_full(buf));
+    }
+  } else if (warp < 4) {
+    int count = 0;
+    for (int tile = first; tile < tiles; tile += stride, ++count) {
+      const Tile t = tile_at<BN>(a, tile);
+      const int buf = count & 1;
+      const uint32_t acc = tmem + (static_cast<uint32_t>(warp * 32) << 16) + buf * BN;
+      const Epilogue ep(a, t.n0, warp, lane);
+      bool ok = wait_or_flag(acc_full(buf), (count >> 1) & 1, &B, a.dev_status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (a.splits == 1) {
+        const int cols = min(BN, a.m - t.token0);
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_wait_ld(r);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float v[4] = {__uint_as_float(r[i]), __uint_as_float(r[i + 1]),
+                                __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])};
+            ep.put4(t.token0 + c + i, v);
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(acc_empty(buf));
+      } else {
+        // column c belongs to rank c / own: into that CTA's exchange buffer
+        const int own = BN / a.splits, shift = __ffs(own) - 1;
+        const uint32_t slot = exchange + (rank * own * kRows + warp * 32 + lane) * 4;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_wait_ld(r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int to = (c + i) >> shift, col = (c + i) & (own - 1);
+            st_remote(remote_smem(slot + col * kRows * 4, to), r[i]);
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  if (a.splits > 1) {  // one tile a cluster
+    cluster_sync();
+    if (warp < 4 && first < tiles && B.error == 0) {
+      const Tile t = tile_at<BN>(a, first);
+      const Epilogue ep(a, t.n0, warp, lane);
+      const int own = BN / a.splits;
+      for (int c = 0; c < own; c += 4) {
+        if (t.token0 + rank * own + c >= a.m) break;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int from = 0; from < a.splits; ++from) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] += ld_shared(exchange + ((from * own + c + i) * kRows + warp * 32 + lane) * 4);
+        }
+        ep.put4(t.token0 + rank * own + c, v);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+std::mutex g_attr_mu;
+bool g_attr_done[64] = {false};
+
+template <int BN, bool FP8>
+cudaError_t set_smem_attr() {
+  return cudaFuncSetAttribute(linear_kernel<BN, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              kSmemBudget + 1024);
+}
+
+int ensure_smem_attr(int dev) {
+  if (dev < 0) return B200_ERR_CUDA;
+  if (dev < 64 && g_attr_done[dev]) return B200_OK;
+  std::lock_guard<std::mutex> lk(g_attr_mu);
+  if (dev < 64 && g_attr_done[dev]) return B200_OK;
+  const cudaError_t es[] = {set_smem_attr<32, false>(),  set_smem_attr<64, false>(),
+                            set_smem_attr<128, false>(), set_smem_attr<256, false>(),
+                            set_smem_attr<32, true>(),   set_smem_attr<64, true>(),
+                            set_smem_attr<128, true>(),  set_smem_attr<256, true>()};
+  for (cudaError_t e : es)
+    if (e != cudaSuccess) return b200host::status_from_cuda(e);
+  if (dev < 64) g_attr_done[dev] = true;
+  return B200_OK;
+}
+
+// rows x k elements of `size` bytes, K innermost
+int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t stride,
+                bool fp8, int box_rows) {
+  const int size = fp8 ? 1 : 2;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * size};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kKBytes / size),
+                             static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t es[2] = {1, 1};
+  return b200host::encode_tiled(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                2, const_cast<void*>(base), dims, strides, box, es,
+                                CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS
+             ? B200_OK
+             : B200_ERR_TENSOR_MAP;
+}
+
+// gate and up rows as (k, 16, gate / up, group of 16): a box is a tile's 128 rows
+int encode_gated(CUtensorMap* map, const void* base, int64_t n, int64_t k, int64_t stride,
+                 bool fp8) {
+  const int size = fp8 ? 1 : 2;
+  const cuuint64_t row = static_cast<cuuint64_t>(stride) * size;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(k), 16u, 2u, static_cast<cuuint64_t>(n / 16)};
+  const cuuint64_t strides[3] = {row, row * static_cast<cuuint64_t>(n), row * 16};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(kKBytes / size), 16, 2, 4};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return b200host::encode_tiled(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                4, const_cast<void*>(base), dims, strides, box, es,
+                                CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == CUDA_SUCCESS
+             ? B200_OK
+             : B200_ERR_TENSOR_MAP;
+}
+
+template <int BN, bool FP8>
+cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, int sms,
+                   cudaStream_t stream) {
+  const int stage_bytes = kABytes + BN * kKBytes;
+  const int exchange = a.splits > 1 ? BN * kRows * 4 : 0;
+  a.stages = (kSmemBudget - exchange) / stage_bytes;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
+  const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
+                                : static_cast<int>(tiles < sms ? tiles : sms);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = a.stages * stage_bytes + exchange + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(a.splits);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, linear_kernel<BN, FP8>, tw, tx, a);
+}
+
+template <bool FP8>
+cudaError_t launch_bn(int bn, const CUtensorMap& tw, const CUtensorMap& tx, const LinearArgs& a,
+                      int sms, cudaStream_t stream) {
+  switch (bn) {
+    case 32: return launch<32, FP8>(tw, tx, a, sms, stream);
+    case 64: return launch<64, FP8>(tw, tx, a, sms, stream);
+    case 128: return launch<128, FP8>(tw, tx, a, sms, stream);
+    default: return launch<256, FP8>(tw, tx, a, sms, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+                           int64_t w_stride, const float* w_scale, const void* bias,
+                           const void* residual, int64_t r_stride, void* out, int64_t o_stride,
+                           int m, int n, int k, int fp8, int gated, int activation,
+                           int32_t* dev_status, void* stream) {
+  if (m < 0 || n <= 0 || k <= 0 || n > 0x3fffffff) return B200_ERR_INVALID_ARGUMENT;
+  if (activation < B200_ACT_NONE || activation > B200_ACT_GELU_TANH)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (m == 0) return B200_OK;
+  if (!x || !w || !out) return B200_ERR_INVALID_ARGUMENT;
+  if (fp8 ? !x_scale || !w_scale : x_scale || w_scale) return B200_ERR_INVALID_ARGUMENT;
+  const int64_t unit = fp8 ? 16 : 8;  // elements of 16 bytes
+  if (!b200host::aligned16(x) || !b200host::aligned16(w) || x_stride % unit || w_stride % unit)
+    return B200_ERR_ALIGNMENT;
+  if (x_stride < k || w_stride < k || o_stride < n || (residual && r_stride < n))
+    return B200_ERR_INVALID_ARGUMENT;
+
+  LinearArgs a{};
+  a.x_scale = x_scale;
+  a.w_scale = w_scale;
+  a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.residual = static_cast<const __nv_bfloat16*>(residual);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.r_row = r_stride;
+  a.o_row = o_stride;
+  a.m = m;
+  a.n = n;
+  const int per = fp8 ? 128 : 64;
+  a.k_blocks = (k + per - 1) / per;
+  a.gated = !gated ? 0 : n % 16 == 0 ? 2 : 1;
+  a.act = activation;
+  a.dev_status = dev_status;
+  a.pairs = n % 2 == 0 && o_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0 &&
+            (residual == nullptr ||
+             (r_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(residual) & 3) == 0));
+  const int dev = b200host::current_device();
+  const int sms = b200host::sm_count(dev);
+  if (sms <= 0) return B200_ERR_CUDA;
+  int st = ensure_smem_attr(dev);
+  if (st != B200_OK) return st;
+
+  const int tile_n = gated ? kRows / 2 : kRows;
+  a.n_tiles = (n + tile_n - 1) / tile_n;
+  const int bn = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+  a.m_tiles = (m + bn - 1) / bn;
+  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
+  if (tiles > 0x3fffffff) return B200_ERR_INVALID_ARGUMENT;
+  a.splits = 1;
+  if (bn <= 64)
+    while (a.splits < kMaxSplits && tiles * a.splits * 2 <= sms && a.splits * 4 <= a.k_blocks)
+      a.splits *= 2;
+
+  CUtensorMap tw, tx;
+  if (a.gated == 2)
+    st = encode_gated(&tw, w, n, k, w_stride, fp8 != 0);
+  else
+    st = encode_rows(&tw, w, gated ? 2 * static_cast<int64_t>(n) : n, k, w_stride, fp8 != 0,
+                     gated ? 16 : kRows);
+  if (st == B200_OK) st = encode_rows(&tx, x, m, k, x_stride, fp8 != 0, bn);
+  if (st != B200_OK) return st;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, tw, tx, a, sms, cs)
+                                        : launch_bn<false>(bn, tw, tx, a, sms, cs));
+}

@@ -65,9 +65,17 @@
 
 #include <mutex>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
+
+using b200::mbar_arrive;
+using b200::smem_desc;
+using b200::tc_fence_after;
+using b200::tc_fence_before;
+using b200::tmem_ld32;
+using b200::tmem_wait_ld;
+using b200::umma_commit;
 
 constexpr int kD = 128;
 constexpr int kBM = 128;                    // query rows per tile (one TMEM lane each)
@@ -213,13 +221,6 @@ struct __align__(8) Barriers {
 };
 
 // ---------------------------------------------------------------- tcgen05
-B200_DEVICE uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  // start>>4 [0,14), LBO>>4 [16,30), SBO>>4 [32,46), version 1 [46,48),
-  // base offset 0, layout SWIZZLE_128B (2) at [61,64)
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) |
-         (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
-}
 
 // kind::f16 instruction descriptor: bf16 x bf16 -> f32, M=128, N=n.
 constexpr uint32_t idesc_bf16(uint32_t n, bool b_mn_major) {
@@ -253,12 +254,6 @@ B200_DEVICE void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
       : "memory");
 }
 
-B200_DEVICE void umma_commit(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-      : "memory");
-}
-
 // 5-D tiled tensor load (no multicast), completing on `bar`.
 B200_DEVICE void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
                              int c2, int c3, int c4) {
@@ -267,42 +262,6 @@ B200_DEVICE void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
       " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
       "r"(c4)
-      : "memory");
-}
-
-B200_DEVICE void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-B200_DEVICE void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 32 consecutive TMEM columns of this thread's lane into r[0..31].  The load is
-// asynchronous: the registers are valid only after tmem_wait_ld(r) below.
-B200_DEVICE void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-}
-
-// tcgen05.wait::ld that also "rewrites" r[0..31], so no use of the loaded
-// registers can be scheduled above the wait.
-B200_DEVICE void tmem_wait_ld(uint32_t* r) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
-        "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
-        "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
-        "+r"(r[31])
-      :
       : "memory");
 }
 
@@ -330,10 +289,6 @@ B200_DEVICE void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 
 B200_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-B200_DEVICE void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per pipeline wait
 

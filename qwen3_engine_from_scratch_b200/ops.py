@@ -18,6 +18,11 @@ this module                                 reference (uphome/Qwen3-engine-from-
 ``kv_scatter_slots``                        vLLM-style slot_mapping write (new entry point)
 ``kv_scatter_span``                         the write of PagedKVCache.update
                                             (qwen3/PagedKVcache.py:187-214), host position
+``rms_norm``, ``rms_norm_fp8``              RMSNorm (qwen3/norm.py:22-26) with the residual's
+                                            addition before it (new entry points)
+``linear``, ``quantize_rows_fp8``           the projections and the MLP (new entry points)
+``rotary``, ``rotary_tables``               qwen3/rope.py:88-110, scaled frequencies
+                                            (new entry points)
 ==========================================  ==================================================
 
 The ``triton_*`` names are kept only so existing call sites bind unchanged; no
@@ -57,6 +62,12 @@ __all__ = [
     "clear_device_status",
     "check_device_status",
     "decode_workspace_bytes",
+    "rms_norm",
+    "rms_norm_fp8",
+    "quantize_rows_fp8",
+    "linear",
+    "rotary",
+    "rotary_tables",
 ]
 
 HEAD_DIM = 128
@@ -820,3 +831,266 @@ def flash_attention_prefill_batched(q, k, v, lens, scaling, num_heads, num_kv_he
     _prefill(qf, kf, vf, out.view(B * S, H, D), dev[:B + 1], dev[B + 1:], S, scaling, num_heads,
              H_kv, head_dim, True)
     return out.reshape(B, S, H * D)
+
+
+# ---------------------------------------------------------------------------
+# the decoder layer around the attention: norm, product, rotary positions
+# ---------------------------------------------------------------------------
+
+FP8 = torch.float8_e4m3fn
+
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _check_on(device: torch.device, **tensors) -> None:
+    """Every given tensor on ``device``, and that device the current one (the
+    kernels go to its current stream)."""
+    assert device.type == "cuda", "b200 kernels need CUDA tensors"
+    assert device.index == torch.cuda.current_device(), \
+        "the tensors must be on the current CUDA device"
+    for name, t in tensors.items():
+        assert t is None or t.device == device, f"{name} must be on {device}"
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """(..., n) as (rows, n) with contiguous rows (a copy only where the strides need one)."""
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _out_rows(out, shape, dtype, device, name):
+    """``out`` (checked) or a new tensor, and its (rows, n) view."""
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        assert out.shape == shape and out.dtype == dtype and out.device == device, \
+            f"{name} must be {tuple(shape)} {dtype} on {device}"
+        assert out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1
+                                       and out.stride(0) >= shape[-1]), \
+            f"{name} must have contiguous rows that do not overlap"
+    return out, out if out.dim() == 2 else out.view(-1, shape[-1])
+
+
+def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
+    assert x.dim() >= 1 and x.dtype == torch.bfloat16, "x must be (..., hidden) bf16"
+    hidden = x.shape[-1]
+    assert hidden > 0, "hidden must be positive"
+    _check_on(x.device, weight=weight, residual=residual)
+    if weight is not None:
+        assert weight.shape == (hidden,) and weight.dtype == torch.bfloat16, \
+            "weight must be (hidden,) bf16"
+        weight = weight.contiguous()
+    x2 = _rows(x)
+    rows = x2.shape[0]
+    y, y2 = _out_rows(out, x.shape, FP8 if fp8 else torch.bfloat16, x.device, "out")
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if fp8 else None
+    h = r2 = h2 = None
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == torch.bfloat16, \
+            "residual must have x's shape, bf16"
+        r2 = _rows(residual)
+        h, h2 = _out_rows(residual_out, x.shape, torch.bfloat16, x.device, "residual_out")
+    else:
+        assert residual_out is None, "residual_out needs a residual"
+    st = _native.load().b200_rms_norm(
+        x2.data_ptr(), x2.stride(0), r2.data_ptr() if r2 is not None else None,
+        r2.stride(0) if r2 is not None else 0, weight.data_ptr() if weight is not None else None,
+        y2.data_ptr(), y2.stride(0), scale.data_ptr() if fp8 else None,
+        h2.data_ptr() if h2 is not None else None, h2.stride(0) if h2 is not None else 0,
+        rows, hidden, float(eps), _stream())
+    _native.check(st, what)
+    return (y,) + ((scale,) if fp8 else ()) + ((h,) if h is not None else ())
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
+    """RMS norm of ``x``, after the residual's addition where one is given.
+
+    x, residual: (..., hidden) bf16; weight: (hidden,) bf16.  With
+    h = x + residual in fp32 the result is h / sqrt(mean(h^2) + eps) * weight,
+    rounded once to bf16; with a residual, (result, bf16(h)).  ``residual_out`` may
+    be ``residual`` itself.  (The reference's RMSNorm and addition:
+    qwen3/norm.py:22-26; it rounds the sum to bf16 before the norm.)
+    """
+    got = _norm(x, weight, residual, eps, False, out, residual_out, "b200_rms_norm")
+    return got if residual is not None else got[0]
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
+    """``rms_norm`` with an 8-bit result: (q, scale) or (q, scale, bf16(h)).
+
+    q: (..., hidden) float8_e4m3fn, scale: (...) fp32, one a row:
+    scale = max(max|y|, 1e-12) / 448 and q = e4m3(y / scale).  What ``linear``
+    takes as ``x`` and ``x_scale``.
+    """
+    return _norm(x, weight, residual, eps, True, out, residual_out, "b200_rms_norm")
+
+
+def quantize_rows_fp8(x, out=None):
+    """(..., n) bf16 rows in 8 bits with an fp32 scale a row: (q, scale), as in
+    ``rms_norm_fp8`` without the norm.  For activations and for ``linear``'s
+    weights (a row is an output channel)."""
+    return _norm(x, None, None, 0.0, True, out, None, "b200_rms_norm")
+
+
+def _tma_rows(t: torch.Tensor):
+    """2-D ``t`` with contiguous rows on 16-byte boundaries, and its row stride:
+    ``t`` itself, or a copy with padded rows (a base, width or stride that is no
+    multiple of 16 bytes)."""
+    unit = 16 // t.element_size()
+    rows, n = t.shape
+    wide = (n + unit - 1) // unit * unit
+    if t.data_ptr() % 16 == 0 and (t.stride(1) == 1 or n == 1):
+        if rows == 1:
+            return t, wide
+        if t.stride(0) % unit == 0 and t.stride(0) >= n:
+            return t, t.stride(0)
+    padded = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
+    padded[:, :n].copy_(t)
+    return padded, wide
+
+
+def linear(x, weight, bias=None, activation=None, gated=False, residual=None, out=None,
+           x_scale=None, weight_scale=None):
+    """Matrix product with bias, activation and residual in its epilogue.
+
+    x: (..., k); weight: (n, k), as torch's Linear holds it; both bf16, or both
+    float8_e4m3fn with ``x_scale`` (...) and ``weight_scale`` (n,) fp32 (from
+    ``rms_norm_fp8`` / ``quantize_rows_fp8``).  Returns (..., n) bf16:
+
+        act(x_scale weight_scale (x weight^T) + bias) + residual
+
+    ``gated``: weight holds n gate rows, then n up rows (bias and weight_scale
+    too), and the result is act(gate) * up + residual.  ``activation``: None, "relu",
+    "silu", "gelu" (error function) or "gelu_tanh".  bias: bf16; residual and
+    ``out``: (..., n) bf16, ``out`` may be ``residual``.  Everything between the
+    operands and the one rounding at the end is fp32.  Operands whose rows do
+    not lie on 16-byte boundaries are copied to padded rows first.
+    """
+    assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
+    assert x.dtype in (torch.bfloat16, FP8) and weight.dtype == x.dtype, \
+        "x and weight must both be bf16 or both float8_e4m3fn"
+    assert weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1], \
+        "x must be (..., k) and weight (n, k)"
+    k = weight.shape[1]
+    wide = weight.shape[0]
+    assert k > 0 and wide > 0 and (not gated or wide % 2 == 0), \
+        "weight must not be empty (gated: gate rows and as many up rows)"
+    n = wide // 2 if gated else wide
+    fp8 = x.dtype == FP8
+    device = x.device
+    _check_on(device, weight=weight, bias=bias, residual=residual, x_scale=x_scale,
+              weight_scale=weight_scale)
+    lead = x.shape[:-1]
+    if fp8:
+        assert x_scale is not None and weight_scale is not None, "fp8 operands need their scales"
+        assert x_scale.shape == lead and x_scale.dtype == torch.float32, \
+            "x_scale must be fp32, one for each row of x"
+        assert weight_scale.shape == (wide,) and weight_scale.dtype == torch.float32, \
+            "weight_scale must be fp32, one for each row of weight"
+        x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    else:
+        assert x_scale is None and weight_scale is None, "scales belong to fp8 operands"
+    if bias is not None:
+        assert bias.shape == (wide,) and bias.dtype == torch.bfloat16, \
+            "bias must be bf16, one for each row of weight"
+        bias = bias.contiguous()
+    shape = lead + (n,)
+    r2 = None
+    if residual is not None:
+        assert residual.shape == shape and residual.dtype == torch.bfloat16, \
+            "residual must have the result's shape, bf16"
+        r2 = _rows(residual)
+        if r2.stride(0) < n:       # broadcast rows
+            r2 = r2.contiguous()
+    y, y2 = _out_rows(out, shape, torch.bfloat16, device, "out")
+    (x2, x_stride), (w2, w_stride) = _tma_rows(_rows(x)), _tma_rows(weight)
+    m = x2.shape[0]
+    st = _native.load().b200_linear(
+        x2.data_ptr(), x_stride, x_scale.data_ptr() if fp8 else None,
+        w2.data_ptr(), w_stride, weight_scale.data_ptr() if fp8 else None,
+        bias.data_ptr() if bias is not None else None,
+        r2.data_ptr() if r2 is not None else None, max(n, r2.stride(0)) if r2 is not None else 0,
+        y2.data_ptr(), y2.stride(0) if m > 1 else n, m, n, k, int(fp8), int(gated),
+        ACTIVATIONS[activation], _status_ptr(device), _stream())
+    _native.check(st, "b200_linear")
+    return y
+
+
+def _rotary_view(t, name):
+    """(T, H, D) or (B, H, S, D) as ((B, H, S, D) sizes, (b, h, s) strides)."""
+    assert t.dtype == torch.bfloat16, f"{name} must be bf16"
+    assert t.dim() in (3, 4), f"{name} must be (T, heads, D) or (B, heads, S, D)"
+    if t.dim() == 3:
+        return (1, t.shape[1], t.shape[0]), (0, t.stride(1), t.stride(0))
+    return (t.shape[0], t.shape[1], t.shape[2]), (t.stride(0), t.stride(1), t.stride(2))
+
+
+def _check_positions(positions, shape, plan, device):
+    assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
+    assert positions.shape == shape, f"positions must be {tuple(shape)}"
+    assert plan.turns.device == device, f"the plan must be on {device}"
+
+
+def rotary(q, k, positions, plan, q_out=None, k_out=None):
+    """Rotary positions of q and k by a ``RotaryPlan``: (q_out, k_out).
+
+    q: (T, H, D) with positions (T,), or (B, H, S, D) with positions (B, S);
+    k: the same with its own number of heads, or None; bf16, any strides with a
+    contiguous head.  The first ``plan.rotary_dim`` elements of every head turn, the
+    rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place).
+    Any int32 or int64 position is exact to 2^-31 turns.
+    """
+    D = q.shape[-1]
+    assert plan.rotary_dim <= D, "the plan's rotary_dim exceeds head_dim"
+    _check_on(q.device, k=k, positions=positions, q_out=q_out, k_out=k_out)
+    outs, args = [], []
+    size = None
+    for t, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if t is None:
+            assert out is None, "k_out needs k"
+            outs.append(None)
+            args.append((None, (0, 0, 0), None, (0, 0, 0), 0))
+            continue
+        (b, h, s), _ = _rotary_view(t, name)
+        assert t.dim() == q.dim() and t.shape[-1] == D and size in (None, (b, s)), \
+            "q and k must agree in all but their heads"
+        size = (b, s)
+        if t.stride(-1) != 1:
+            t = t.contiguous()
+        if out is None:
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        assert out.shape == t.shape and out.dtype == t.dtype and out.stride(-1) == 1, \
+            f"{name}_out must be like {name} with a contiguous head"
+        outs.append(out)
+        args.append((t.data_ptr(), _rotary_view(t, name)[1], out.data_ptr(),
+                     _rotary_view(out, name)[1], h))
+    b, s = size
+    _check_positions(positions, (s,) if q.dim() == 3 else (b, s), plan, q.device)
+    (qp, qs, qop, qos, hq), (kp, ks, kop, kos, hk) = args
+    st = _native.load().b200_rotary(
+        qp, *qs, kp, *ks, qop, *qos, kop, *kos, positions.data_ptr(),
+        positions.stride(0) if q.dim() == 4 else 0, positions.stride(-1),
+        int(positions.dtype == torch.int64), plan.turns.data_ptr(), plan.gain, b, s, hq, hk, D,
+        plan.rotary_dim, int(plan.interleaved), _stream())
+    _native.check(st, "b200_rotary")
+    return tuple(outs)
+
+
+def rotary_tables(positions, plan):
+    """(cos, sin) of a plan at ``positions`` (S,) or (B, S): fp32 (..., rotary_dim)
+    rows with each pair's value at both of its elements, as
+    ``qk_norm_rope_kv_write`` takes them (half layout, rotary_dim == head_dim)."""
+    assert positions.dim() in (1, 2), "positions must be (S,) or (B, S)"
+    _check_on(positions.device)
+    _check_positions(positions, positions.shape, plan, positions.device)
+    b, s = (1, positions.shape[0]) if positions.dim() == 1 else positions.shape
+    cos = torch.empty(tuple(positions.shape) + (plan.rotary_dim,), dtype=torch.float32,
+                      device=positions.device)
+    sin = torch.empty_like(cos)
+    st = _native.load().b200_rotary_tables(
+        positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
+        positions.stride(-1), int(positions.dtype == torch.int64), plan.turns.data_ptr(),
+        plan.gain, cos.data_ptr(), sin.data_ptr(), b, s, plan.rotary_dim, int(plan.interleaved),
+        _stream())
+    _native.check(st, "b200_rotary_tables")
+    return cos, sin
