@@ -10,10 +10,11 @@
 // 128-row tiles and pads only the small token side, and one kernel serves one
 // token and thousands.  Token tiles of BN columns; two accumulators of BN
 // columns, so the epilogue of one tile overlaps the product of the next.
-//   warps 0-3  epilogue: lane l of warp w owns accumulator lane 32 w + l
-//   warp 4     TMA producer (one lane): 128-byte swizzled K-major tiles,
+//   warps 0-7  epilogue: lane l of warp w owns accumulator lane 32 (w % 4) + l,
+//              of every other 32 token columns
+//   warp 8     TMA producer (one lane): 128-byte swizzled K-major tiles,
 //              128 weight rows and BN tokens x 128 bytes of K a stage
-//   warp 5     MMA issuer (one lane): 4 instructions a stage (K = 32 bytes)
+//   warp 9     MMA issuer (one lane): 4 instructions a stage (K = 32 bytes)
 // Gated: lanes 0-15 of every warp hold gate rows and lanes 16-31 the up rows
 // of the same 16 outputs, so the two meet by one shuffle; the tile's rows
 // come from one 4-D box (k, 16, gate/up, group) where n is a multiple of 16, or
@@ -39,10 +40,11 @@ using namespace b200;
 constexpr int kRows = 128;        // weight rows of a tile (TMEM lanes)
 constexpr int kKBytes = 128;      // bytes of K a stage: one swizzle row
 constexpr int kABytes = kRows * kKBytes;
-constexpr int kThreads = 192;
-constexpr int kEpilogueThreads = 128;
-constexpr int kProducerWarp = 4;
-constexpr int kMmaWarp = 5;
+constexpr int kThreads = 320;
+constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueThreads = kEpilogueWarps * 32;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
 constexpr int kMaxStages = 10;
 constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
 constexpr int kMaxSplits = 8;
@@ -124,16 +126,30 @@ B200_DEVICE float ld_shared(uint32_t addr) {
   return v;
 }
 
-B200_DEVICE float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+// v / (1 + e^-v'): the quotient stays right at both ends (v' large and negative: 0)
+B200_DEVICE float gate_by(float v, float z) { return __fdividef(v, 1.0f + __expf(-z)); }
 
-B200_DEVICE float activate(float v, int act) {
-  switch (act) {
-    case B200_ACT_RELU: return v < 0.0f ? 0.0f : v;  // NaN stays
-    case B200_ACT_SILU: return v * sigmoid(v);
-    case B200_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    case B200_ACT_GELU_TANH:  // (1 + tanh z) / 2 = sigmoid(2 z)
-      return v * sigmoid(1.5957691216057308f * (v + 0.044715f * v * v * v));
-    default: return v;
+template <int N>
+B200_DEVICE void activate(float (&v)[N], int act) {
+  switch (act) {  // outside the loops: one branch for N values
+    case B200_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // NaN stays
+      break;
+    case B200_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = gate_by(v[i], v[i]);
+      break;
+    case B200_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
+      break;
+    case B200_ACT_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + e^-2z)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = gate_by(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+      break;
+    default: break;
   }
 }
 
@@ -158,17 +174,23 @@ B200_DEVICE Tile tile_at(const LinearArgs& a, int tile) {
 }
 
 // A lane's share of the epilogue of a tile: turns raw accumulators of this
-// lane's row into outputs.
+// lane's row into outputs.  Whole tiles take stores without bounds checks.
 struct Epilogue {
   const LinearArgs& a;
   int lane, row_n;   // output column of this lane
   int pair_n;        // first of the two output columns this lane writes
+  bool odd, high;    // odd lane of a pair / upper half-warp
+  bool whole;        // every column of the tile exists, 4-byte stores are aligned
   float w_scale, bias;
 
   B200_DEVICE Epilogue(const LinearArgs& args, int n0, int warp, int l) : a(args), lane(l) {
-    row_n = a.gated ? n0 + warp * 16 + (l & 15) : n0 + warp * 32 + l;
+    const int quarter = warp & 3;
+    row_n = a.gated ? n0 + quarter * 16 + (l & 15) : n0 + quarter * 32 + l;
     pair_n = row_n & ~1;
-    const int w_row = a.gated && l >= 16 ? a.n + row_n : row_n;
+    odd = l & 1;
+    high = l >= 16;
+    whole = a.pairs && n0 + (a.gated ? kRows / 2 : kRows) <= a.n;
+    const int w_row = a.gated && high ? a.n + row_n : row_n;
     const bool live = row_n < a.n;
     w_scale = a.w_scale != nullptr && live ? a.w_scale[w_row] : 1.0f;
     bias = a.bias != nullptr && live ? __bfloat162float(a.bias[w_row]) : 0.0f;
@@ -180,58 +202,90 @@ struct Epilogue {
     __nv_bfloat16* o = a.out + token * a.o_row + pair_n;
     const __nv_bfloat16* r =
         a.residual != nullptr ? a.residual + token * a.r_row + pair_n : nullptr;
-    if (a.pairs) {
-      if (r != nullptr) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(r);
-        lo += bf16_lo(w);
-        hi += bf16_hi(w);
-      }
-      *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(lo, hi);
-    } else {
-      if (r != nullptr) lo += __bfloat162float(r[0]);
-      o[0] = __float2bfloat16_rn(lo);
-      if (pair_n + 1 < a.n) {
-        if (r != nullptr) hi += __bfloat162float(r[1]);
-        o[1] = __float2bfloat16_rn(hi);
+    if (r != nullptr) lo += __bfloat162float(r[0]);
+    o[0] = __float2bfloat16_rn(lo);
+    if (pair_n + 1 < a.n) {
+      if (r != nullptr) hi += __bfloat162float(r[1]);
+      o[1] = __float2bfloat16_rn(hi);
+    }
+  }
+
+  // Values v[0..N) of this lane for the tokens token, token + step, ...: lanes
+  // 2i and 2i + 1 swap every other one, so that the even lane holds both
+  // outputs of the even tokens and the odd lane those of the odd ones.
+  template <int N>
+  B200_DEVICE void put_all(int token, int step, const float (&v)[N],
+                           const uint32_t (&res)[N / 2], bool fast) const {
+    const int first = token + (odd ? step : 0);
+    __nv_bfloat16* o = a.out + first * a.o_row + pair_n;
+    const int64_t jump = 2 * step * a.o_row;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+      float lo = odd ? got : v[i], hi = odd ? v[i + 1] : got;
+      if (fast) {
+        if (a.residual != nullptr) {
+          lo += bf16_lo(res[i / 2]);
+          hi += bf16_hi(res[i / 2]);
+        }
+        *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(lo, hi);
+        o += jump;
+      } else {
+        put(first + i * step, lo, hi);
       }
     }
   }
 
-  // this lane's v0 of `token` and v1 of `token + step`: the even lane of a
-  // pair writes the first token's two outputs, the odd lane the second's
-  B200_DEVICE void put_pair(int token, int step, float v0, float v1) const {
-    const bool odd = lane & 1;
-    const float got = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
-    put(odd ? token + step : token, odd ? got : v0, odd ? v1 : got);
-  }
-
-  // accumulators of tokens token .. token + 3
-  B200_DEVICE void put4(int token, const float (&acc)[4]) const {
-    float v[4];
+  // accumulators of the tokens token .. token + N - 1; xs: their scales
+  template <int N, class Wait>
+  B200_DEVICE void put_columns(int token, float (&v)[N], const float* xs, Wait&& wait) const {
+    const bool fast = whole && token + N <= a.m;
+    constexpr int kMost = N / 2;
+    uint32_t res[kMost];
+    if (a.residual != nullptr && fast) {
+      // the residual's words of this lane, read while the accumulators come
+      const int step = a.gated ? 2 : 1;
+      const int first = token + (a.gated && high ? 1 : 0) + (odd ? step : 0);
+      const __nv_bfloat16* r = a.residual + first * a.r_row + pair_n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = acc[i];
-      if (a.x_scale != nullptr)
-        v[i] *= w_scale * (token + i < a.m ? __ldg(a.x_scale + token + i) : 0.0f);
-      v[i] += bias;
+      for (int i = 0; i < kMost; ++i)
+        if (!a.gated || i < kMost / 2)
+          res[i] = *reinterpret_cast<const uint32_t*>(r + 2 * i * step * a.r_row);
+    }
+    wait();
+    if (a.w_scale != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(xs + i);
+        v[i] *= w_scale * s.x;
+        v[i + 1] *= w_scale * s.y;
+        v[i + 2] *= w_scale * s.z;
+        v[i + 3] *= w_scale * s.w;
+      }
+    }
+    if (a.bias != nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += bias;
     }
     if (a.gated) {
       // low half-warp: gate, high half-warp: up; each keeps one token of two
-      const bool high = lane >= 16;
-      float o[2];
+      float gate[N / 2], up[N / 2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < N / 2; ++i) {
         const float got = __shfl_xor_sync(0xffffffffu, high ? v[2 * i] : v[2 * i + 1], 16);
-        const float gate = high ? got : v[2 * i];
-        const float up = high ? v[2 * i + 1] : got;
-        o[i] = activate(gate, a.act) * up;
+        gate[i] = high ? got : v[2 * i];
+        up[i] = high ? v[2 * i + 1] : got;
       }
-      put_pair(token + (high ? 1 : 0), 2, o[0], o[1]);
-    } else {
+      activate(gate, a.act);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = activate(v[i], a.act);
-      put_pair(token, 1, v[0], v[1]);
-      put_pair(token + 2, 1, v[2], v[3]);
+      for (int i = 0; i < N / 2; ++i) gate[i] *= up[i];
+      uint32_t half[N / 4];
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) half[i] = res[i];
+      put_all<N / 2>(token + (high ? 1 : 0), 2, gate, half, fast);
+    } else {
+      activate(v, a.act);
+      put_all<N>(token, 1, v, res, fast);
     }
   }
 };
@@ -242,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers B;
+  __shared__ __align__(16) float xs[kEpilogueWarps][32];  // token scales of a warp's columns
   constexpr int kBBytes = BN * kKBytes;
   constexpr int kStageBytes = kABytes + kBBytes;
   constexpr int kKElems = FP8 ? 128 : 64;
@@ -359,12 +414,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) umma_commit(acc_full(buf));
     }
-  } else if (warp < 4) {
+  } else if (warp < kEpilogueWarps) {
+    const int part = warp >> 2;  // which of every two 32-column groups
+    const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
       const Tile t = tile_at<BN>(a, tile);
       const int buf = count & 1;
-      const uint32_t acc = tmem + (static_cast<uint32_t>(warp * 32) << 16) + buf * BN;
+      const uint32_t acc = tmem + lane0 + buf * BN;
       const Epilogue ep(a, t.n0, warp, lane);
       bool ok = wait_or_flag(acc_full(buf), (count >> 1) & 1, &B, a.dev_status);
       ok = __all_sync(0xffffffffu, ok);
@@ -373,25 +430,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (a.splits == 1) {
         const int cols = min(BN, a.m - t.token0);
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(acc + c, r);
-          tmem_wait_ld(r);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float v[4] = {__uint_as_float(r[i]), __uint_as_float(r[i + 1]),
-                                __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])};
-            ep.put4(t.token0 + c + i, v);
+        for (int c = part * 32; c < cols; c += 64) {
+          float v[32];
+          tmem_ld32(acc + c, reinterpret_cast<uint32_t*>(v));
+          if (a.w_scale != nullptr) {
+            __syncwarp();
+            xs[warp][lane] = c + lane < cols ? a.x_scale[t.token0 + c + lane] : 0.0f;
+            __syncwarp();
           }
+          ep.put_columns<32>(t.token0 + c, v, xs[warp],
+                             [&] { tmem_wait_ld(reinterpret_cast<uint32_t*>(v)); });
         }
         tc_fence_before();
         mbar_arrive(acc_empty(buf));
       } else {
         // column c belongs to rank c / own: into that CTA's exchange buffer
         const int own = BN / a.splits, shift = __ffs(own) - 1;
-        const uint32_t slot = exchange + (rank * own * kRows + warp * 32 + lane) * 4;
+        const uint32_t slot = exchange + (rank * own * kRows + (warp & 3) * 32 + lane) * 4;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = part * 32; c < BN; c += 64) {
           uint32_t r[32];
           tmem_ld32(acc + c, r);
           tmem_wait_ld(r);
@@ -408,19 +465,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   if (a.splits > 1) {  // one tile a cluster
     cluster_sync();
-    if (warp < 4 && first < tiles && B.error == 0) {
+    if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
       const Tile t = tile_at<BN>(a, first);
       const Epilogue ep(a, t.n0, warp, lane);
       const int own = BN / a.splits;
-      for (int c = 0; c < own; c += 4) {
-        if (t.token0 + rank * own + c >= a.m) break;
+      const int token0 = t.token0 + rank * own;
+      for (int c = (warp >> 2) * 4; c < own; c += 8) {
+        if (token0 + c >= a.m) break;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int from = 0; from < a.splits; ++from) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            v[i] += ld_shared(exchange + ((from * own + c + i) * kRows + warp * 32 + lane) * 4);
+            v[i] += ld_shared(exchange + ((from * own + c + i) * kRows + (warp & 3) * 32 + lane) * 4);
         }
-        ep.put4(t.token0 + rank * own + c, v);
+        if (a.w_scale != nullptr) {
+          __syncwarp();
+          if (lane < 4) xs[warp][lane] = token0 + c + lane < a.m ? a.x_scale[token0 + c + lane] : 0.0f;
+          __syncwarp();
+        }
+        ep.put_columns<4>(token0 + c, v, xs[warp], [] {});
       }
     }
   }

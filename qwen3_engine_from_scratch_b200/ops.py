@@ -842,64 +842,88 @@ FP8 = torch.float8_e4m3fn
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
-def _check_on(device: torch.device, **tensors) -> None:
-    """Every given tensor on ``device``, and that device the current one (the
-    kernels go to its current stream)."""
-    assert device.type == "cuda", "b200 kernels need CUDA tensors"
-    assert device.index == torch.cuda.current_device(), \
-        "the tensors must be on the current CUDA device"
-    for name, t in tensors.items():
-        assert t is None or t.device == device, f"{name} must be on {device}"
+def _gpu_of(x: torch.Tensor, *others) -> int:
+    """The index of x's device: the current CUDA device (the kernels go to its
+    current stream), where every other given tensor lies too.  (Single calls of
+    these operators are bound by the host, so the checks use the cheap accessors.)"""
+    index = x.get_device()
+    assert index >= 0, "b200 kernels need CUDA tensors"
+    assert index == torch.cuda.current_device(), "the tensors must be on the current CUDA device"
+    for t in others:
+        assert t is None or t.get_device() == index, f"every tensor must be on cuda:{index}"
+    return index
+
+
+def _stream_of(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """(..., n) as (rows, n) with contiguous rows (a copy only where the strides need one)."""
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _out_rows(out, shape, dtype, device, name):
-    """``out`` (checked) or a new tensor, and its (rows, n) view."""
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-    else:
-        assert out.shape == shape and out.dtype == dtype and out.device == device, \
-            f"{name} must be {tuple(shape)} {dtype} on {device}"
-        assert out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1
-                                       and out.stride(0) >= shape[-1]), \
-            f"{name} must have contiguous rows that do not overlap"
-    return out, out if out.dim() == 2 else out.view(-1, shape[-1])
+def _out_rows(out, shape, dtype, index, name):
+    """The (rows, n) view of a caller's output, checked."""
+    assert out.shape == shape and out.dtype == dtype and out.get_device() == index, \
+        f"{name} must be {tuple(shape)} {dtype} on cuda:{index}"
+    assert out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1
+                                   and out.stride(0) >= shape[-1]), \
+        f"{name} must have contiguous rows that do not overlap"
+    return out if out.dim() == 2 else out.view(-1, shape[-1])
 
 
 def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
-    assert x.dim() >= 1 and x.dtype == torch.bfloat16, "x must be (..., hidden) bf16"
-    hidden = x.shape[-1]
+    shape = x.shape
+    assert x.dtype == torch.bfloat16 and len(shape) >= 1, "x must be (..., hidden) bf16"
+    hidden = shape[-1]
     assert hidden > 0, "hidden must be positive"
-    _check_on(x.device, weight=weight, residual=residual)
+    index = _gpu_of(x, weight, residual)
+    w_ptr = None
     if weight is not None:
-        assert weight.shape == (hidden,) and weight.dtype == torch.bfloat16, \
-            "weight must be (hidden,) bf16"
-        weight = weight.contiguous()
+        assert weight.dim() == 1 and weight.shape[0] == hidden and \
+            weight.dtype == torch.bfloat16, "weight must be (hidden,) bf16"
+        if weight.stride(0) != 1:
+            weight = weight.contiguous()
+        w_ptr = weight.data_ptr()
     x2 = _rows(x)
     rows = x2.shape[0]
-    y, y2 = _out_rows(out, x.shape, FP8 if fp8 else torch.bfloat16, x.device, "out")
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if fp8 else None
-    h = r2 = h2 = None
+    if out is None:
+        y = x.new_empty(shape, dtype=FP8) if fp8 else \
+            torch.empty_like(x, memory_format=torch.contiguous_format)
+        y_stride = hidden
+    else:
+        y, y_stride = out, _out_rows(out, shape, FP8 if fp8 else torch.bfloat16, index,
+                                     "out").stride(0)
+    scale = s_ptr = None
+    if fp8:
+        scale = x.new_empty(shape[:-1], dtype=torch.float32)
+        s_ptr = scale.data_ptr()
+    h = r2 = r_ptr = h_ptr = None
+    r_stride = h_stride = 0
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype == torch.bfloat16, \
+        assert residual.shape == shape and residual.dtype == torch.bfloat16, \
             "residual must have x's shape, bf16"
         r2 = _rows(residual)
-        h, h2 = _out_rows(residual_out, x.shape, torch.bfloat16, x.device, "residual_out")
+        r_ptr, r_stride = r2.data_ptr(), r2.stride(0)
+        if residual_out is None:
+            h, h_stride = torch.empty_like(x, memory_format=torch.contiguous_format), hidden
+        else:
+            h, h_stride = residual_out, _out_rows(residual_out, shape, torch.bfloat16, index,
+                                                  "residual_out").stride(0)
+        h_ptr = h.data_ptr()
     else:
         assert residual_out is None, "residual_out needs a residual"
-    st = _native.load().b200_rms_norm(
-        x2.data_ptr(), x2.stride(0), r2.data_ptr() if r2 is not None else None,
-        r2.stride(0) if r2 is not None else 0, weight.data_ptr() if weight is not None else None,
-        y2.data_ptr(), y2.stride(0), scale.data_ptr() if fp8 else None,
-        h2.data_ptr() if h2 is not None else None, h2.stride(0) if h2 is not None else 0,
-        rows, hidden, float(eps), _stream())
-    _native.check(st, what)
-    return (y,) + ((scale,) if fp8 else ()) + ((h,) if h is not None else ())
+    st = _native.load().b200_rms_norm(x2.data_ptr(), x2.stride(0), r_ptr, r_stride, w_ptr,
+                                      y.data_ptr(), y_stride, s_ptr, h_ptr, h_stride, rows, hidden,
+                                      eps, _stream_of(index))
+    if st:
+        _native.check(st, what)
+    if fp8:
+        return (y, scale) if h is None else (y, scale, h)
+    return y if h is None else (y, h)
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
@@ -911,8 +935,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     be ``residual`` itself.  (The reference's RMSNorm and addition:
     qwen3/norm.py:22-26; it rounds the sum to bf16 before the norm.)
     """
-    got = _norm(x, weight, residual, eps, False, out, residual_out, "b200_rms_norm")
-    return got if residual is not None else got[0]
+    return _norm(x, weight, residual, eps, False, out, residual_out, "b200_rms_norm")
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
@@ -967,68 +990,81 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     not lie on 16-byte boundaries are copied to padded rows first.
     """
     assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
-    assert x.dtype in (torch.bfloat16, FP8) and weight.dtype == x.dtype, \
+    dtype = x.dtype
+    fp8 = dtype == FP8
+    assert (fp8 or dtype == torch.bfloat16) and weight.dtype == dtype, \
         "x and weight must both be bf16 or both float8_e4m3fn"
+    lead = x.shape[:-1]
     assert weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1], \
         "x must be (..., k) and weight (n, k)"
-    k = weight.shape[1]
-    wide = weight.shape[0]
+    wide, k = weight.shape
     assert k > 0 and wide > 0 and (not gated or wide % 2 == 0), \
         "weight must not be empty (gated: gate rows and as many up rows)"
     n = wide // 2 if gated else wide
-    fp8 = x.dtype == FP8
-    device = x.device
-    _check_on(device, weight=weight, bias=bias, residual=residual, x_scale=x_scale,
-              weight_scale=weight_scale)
-    lead = x.shape[:-1]
+    index = _gpu_of(x, weight, bias, residual, x_scale, weight_scale)
+    xs_ptr = ws_ptr = b_ptr = r_ptr = None
     if fp8:
         assert x_scale is not None and weight_scale is not None, "fp8 operands need their scales"
         assert x_scale.shape == lead and x_scale.dtype == torch.float32, \
             "x_scale must be fp32, one for each row of x"
-        assert weight_scale.shape == (wide,) and weight_scale.dtype == torch.float32, \
+        assert weight_scale.dim() == 1 and weight_scale.shape[0] == wide and \
+            weight_scale.dtype == torch.float32, \
             "weight_scale must be fp32, one for each row of weight"
         x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+        xs_ptr, ws_ptr = x_scale.data_ptr(), weight_scale.data_ptr()
     else:
         assert x_scale is None and weight_scale is None, "scales belong to fp8 operands"
     if bias is not None:
-        assert bias.shape == (wide,) and bias.dtype == torch.bfloat16, \
+        assert bias.dim() == 1 and bias.shape[0] == wide and bias.dtype == torch.bfloat16, \
             "bias must be bf16, one for each row of weight"
         bias = bias.contiguous()
+        b_ptr = bias.data_ptr()
     shape = lead + (n,)
-    r2 = None
+    r_stride = 0
     if residual is not None:
         assert residual.shape == shape and residual.dtype == torch.bfloat16, \
             "residual must have the result's shape, bf16"
         r2 = _rows(residual)
-        if r2.stride(0) < n:       # broadcast rows
+        if r2.shape[0] > 1 and r2.stride(0) < n:       # broadcast rows
             r2 = r2.contiguous()
-    y, y2 = _out_rows(out, shape, torch.bfloat16, device, "out")
+        r_ptr, r_stride = r2.data_ptr(), max(n, r2.stride(0))
+    if out is None:
+        y, y_stride = x.new_empty(shape, dtype=torch.bfloat16), n
+    else:
+        y, y_stride = out, max(n, _out_rows(out, shape, torch.bfloat16, index, "out").stride(0))
     (x2, x_stride), (w2, w_stride) = _tma_rows(_rows(x)), _tma_rows(weight)
-    m = x2.shape[0]
     st = _native.load().b200_linear(
-        x2.data_ptr(), x_stride, x_scale.data_ptr() if fp8 else None,
-        w2.data_ptr(), w_stride, weight_scale.data_ptr() if fp8 else None,
-        bias.data_ptr() if bias is not None else None,
-        r2.data_ptr() if r2 is not None else None, max(n, r2.stride(0)) if r2 is not None else 0,
-        y2.data_ptr(), y2.stride(0) if m > 1 else n, m, n, k, int(fp8), int(gated),
-        ACTIVATIONS[activation], _status_ptr(device), _stream())
-    _native.check(st, "b200_linear")
+        x2.data_ptr(), x_stride, xs_ptr, w2.data_ptr(), w_stride, ws_ptr, b_ptr, r_ptr, r_stride,
+        y.data_ptr(), y_stride, x2.shape[0], n, k, fp8, gated, ACTIVATIONS[activation],
+        _status_ptr(x.device), _stream_of(index))
+    if st:
+        _native.check(st, "b200_linear")
     return y
 
 
-def _rotary_view(t, name):
-    """(T, H, D) or (B, H, S, D) as ((B, H, S, D) sizes, (b, h, s) strides)."""
-    assert t.dtype == torch.bfloat16, f"{name} must be bf16"
-    assert t.dim() in (3, 4), f"{name} must be (T, heads, D) or (B, heads, S, D)"
-    if t.dim() == 3:
-        return (1, t.shape[1], t.shape[0]), (0, t.stride(1), t.stride(0))
-    return (t.shape[0], t.shape[1], t.shape[2]), (t.stride(0), t.stride(1), t.stride(2))
+def _rotary_head(t, out, dims, name):
+    """Pointers, (b, h, s) strides and heads of q or k and its output."""
+    shape = t.shape
+    assert t.dtype == torch.bfloat16 and len(shape) == dims, \
+        f"{name} must be bf16, (T, heads, D) or (B, heads, S, D) like q"
+    if t.stride(-1) != 1:
+        t = t.contiguous()
+    if out is None:
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    else:
+        assert out.shape == shape and out.dtype == t.dtype and out.stride(-1) == 1, \
+            f"{name}_out must be like {name} with a contiguous head"
+    if dims == 3:
+        (s0, h0, _), (s1, h1, _) = t.stride(), out.stride()
+        b0 = b1 = 0
+    else:
+        (b0, h0, s0, _), (b1, h1, s1, _) = t.stride(), out.stride()
+    return t, out, (t.data_ptr(), b0, h0, s0), (out.data_ptr(), b1, h1, s1), shape[1]
 
 
-def _check_positions(positions, shape, plan, device):
+def _check_positions(positions, plan, index):
     assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
-    assert positions.shape == shape, f"positions must be {tuple(shape)}"
-    assert plan.turns.device == device, f"the plan must be on {device}"
+    assert plan.turns.get_device() == index, f"the plan must be on cuda:{index}"
 
 
 def rotary(q, k, positions, plan, q_out=None, k_out=None):
@@ -1040,40 +1076,31 @@ def rotary(q, k, positions, plan, q_out=None, k_out=None):
     rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place).
     Any int32 or int64 position is exact to 2^-31 turns.
     """
-    D = q.shape[-1]
+    dims, D = q.dim(), q.shape[-1]
+    assert dims in (3, 4), "q must be (T, heads, D) or (B, heads, S, D)"
     assert plan.rotary_dim <= D, "the plan's rotary_dim exceeds head_dim"
-    _check_on(q.device, k=k, positions=positions, q_out=q_out, k_out=k_out)
-    outs, args = [], []
-    size = None
-    for t, out, name in ((q, q_out, "q"), (k, k_out, "k")):
-        if t is None:
-            assert out is None, "k_out needs k"
-            outs.append(None)
-            args.append((None, (0, 0, 0), None, (0, 0, 0), 0))
-            continue
-        (b, h, s), _ = _rotary_view(t, name)
-        assert t.dim() == q.dim() and t.shape[-1] == D and size in (None, (b, s)), \
+    index = _gpu_of(q, k, positions, q_out, k_out)
+    batch, seq = (1, q.shape[0]) if dims == 3 else (q.shape[0], q.shape[2])
+    q, q_out, q_in_args, q_out_args, heads = _rotary_head(q, q_out, dims, "q")
+    k_in_args = k_out_args = (None, 0, 0, 0)
+    kv_heads = 0
+    if k is not None:
+        k, k_out, k_in_args, k_out_args, kv_heads = _rotary_head(k, k_out, dims, "k")
+        assert k.shape[-1] == D and k.shape[0] == q.shape[0] and k.shape[-2 if dims == 4 else 0] == seq, \
             "q and k must agree in all but their heads"
-        size = (b, s)
-        if t.stride(-1) != 1:
-            t = t.contiguous()
-        if out is None:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        assert out.shape == t.shape and out.dtype == t.dtype and out.stride(-1) == 1, \
-            f"{name}_out must be like {name} with a contiguous head"
-        outs.append(out)
-        args.append((t.data_ptr(), _rotary_view(t, name)[1], out.data_ptr(),
-                     _rotary_view(out, name)[1], h))
-    b, s = size
-    _check_positions(positions, (s,) if q.dim() == 3 else (b, s), plan, q.device)
-    (qp, qs, qop, qos, hq), (kp, ks, kop, kos, hk) = args
+    else:
+        assert k_out is None, "k_out needs k"
+    _check_positions(positions, plan, index)
+    assert tuple(positions.shape) == ((seq,) if dims == 3 else (batch, seq)), \
+        "positions must be (T,), or (B, S) for 4-D q"
     st = _native.load().b200_rotary(
-        qp, *qs, kp, *ks, qop, *qos, kop, *kos, positions.data_ptr(),
-        positions.stride(0) if q.dim() == 4 else 0, positions.stride(-1),
-        int(positions.dtype == torch.int64), plan.turns.data_ptr(), plan.gain, b, s, hq, hk, D,
-        plan.rotary_dim, int(plan.interleaved), _stream())
-    _native.check(st, "b200_rotary")
-    return tuple(outs)
+        *q_in_args, *k_in_args, *q_out_args, *k_out_args, positions.data_ptr(),
+        positions.stride(0) if dims == 4 else 0, positions.stride(-1),
+        positions.dtype == torch.int64, plan.turns.data_ptr(), plan.gain, batch, seq, heads, kv_heads, D,
+        plan.rotary_dim, plan.interleaved, _stream_of(index))
+    if st:
+        _native.check(st, "b200_rotary")
+    return q_out, k_out
 
 
 def rotary_tables(positions, plan):
@@ -1081,8 +1108,8 @@ def rotary_tables(positions, plan):
     rows with each pair's value at both of its elements, as
     ``qk_norm_rope_kv_write`` takes them (half layout, rotary_dim == head_dim)."""
     assert positions.dim() in (1, 2), "positions must be (S,) or (B, S)"
-    _check_on(positions.device)
-    _check_positions(positions, positions.shape, plan, positions.device)
+    index = _gpu_of(positions)
+    _check_positions(positions, plan, index)
     b, s = (1, positions.shape[0]) if positions.dim() == 1 else positions.shape
     cos = torch.empty(tuple(positions.shape) + (plan.rotary_dim,), dtype=torch.float32,
                       device=positions.device)
@@ -1091,6 +1118,6 @@ def rotary_tables(positions, plan):
         positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
         positions.stride(-1), int(positions.dtype == torch.int64), plan.turns.data_ptr(),
         plan.gain, cos.data_ptr(), sin.data_ptr(), b, s, plan.rotary_dim, int(plan.interleaved),
-        _stream())
+        _stream_of(index))
     _native.check(st, "b200_rotary_tables")
     return cos, sin

@@ -88,7 +88,6 @@ class RotaryPlan:
         self.turns = torch.tensor([_signed64(round(f / (2 * math.pi) * 2.0 ** 64)) for f in self.freq],
                                   dtype=torch.int64, device=device)
 
-
 def _signed64(v):
     v &= (1 << 64) - 1
     return v - (1 << 64) if v >> 63 else v
