@@ -42,14 +42,14 @@ constexpr int kKBytes = 128;      // bytes of K a stage: one swizzle row
 constexpr int kABytes = kRows * kKBytes;
 constexpr int kThreads = 320;
 constexpr int kEpilogueWarps = 8;
-constexpr int kEpilogueThreads = kEpilogueWarps * 32;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kMaxStages = 10;
 constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
 constexpr int kMaxSplits = 8;
 constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
-constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s a pipeline wait
+constexpr uint64_t kDrainLimitNs = 100000000ull;   // 0.1 s a copy after a give-up
 
 struct LinearArgs {
   const float* x_scale;  // nullable together
@@ -84,18 +84,34 @@ B200_DEVICE bool wait_or_flag(uint32_t bar, uint32_t parity, Barriers* B, int32_
 
 // c format f32, a / b format bf16 (1) of kind::f16 or e4m3 (0) of kind::f8f6f4, both K-major
 template <bool FP8>
-constexpr uint32_t instruction(uint32_t n) {
+constexpr uint32_t instruction(uint32_t m, uint32_t n) {
   return (1u << 4) | ((FP8 ? 0u : 1u) << 7) | ((FP8 ? 0u : 1u) << 10) | ((n >> 3) << 17) |
-         ((static_cast<uint32_t>(kRows) >> 4) << 24);
+         ((m >> 4) << 24);
 }
 
-template <bool FP8>
+// PAIR: the two CTAs of a cluster work as one (cta_group::2), rows 0-127 of A
+// and the first half of B in the first CTA's shared memory, the rest in the second's
+template <bool FP8, bool PAIR>
 B200_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (FP8) {
+  if constexpr (FP8 && PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else if constexpr (FP8) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else if constexpr (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
   } else {
@@ -108,6 +124,73 @@ B200_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_
   }
 }
 
+// every MMA issued so far by this thread is done: an arrival on `bar` (PAIR: on
+// the barrier at that place in both CTAs)
+template <bool PAIR>
+B200_DEVICE void commit(uint32_t bar) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  } else {
+    umma_commit(bar);
+  }
+}
+
+// Tiled loads of this GPU's memory into this CTA (no multicast); PAIR: `bar` may lie
+// in the other CTA of the pair.
+template <bool PAIR>
+B200_DEVICE void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+  } else {
+    tma_load_2d(dst, map, bar, c0, c1);
+  }
+}
+template <bool PAIR>
+B200_DEVICE void load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                         int c3) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+  } else {
+    tma_load_4d_nohint(dst, map, bar, c0, c1, c2, c3);
+  }
+}
+
+template <bool PAIR>
+B200_DEVICE void tmem_alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR>
+B200_DEVICE void tmem_dealloc(uint32_t tmem, uint32_t cols) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols)
+                 : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols)
+                 : "memory");
+}
+
 B200_DEVICE void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -116,6 +199,10 @@ B200_DEVICE uint32_t remote_smem(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
+}
+// an arrival on a barrier of any CTA of the cluster
+B200_DEVICE void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 B200_DEVICE void st_remote(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
@@ -160,8 +247,10 @@ struct Tile {
 // Tiles in groups of kGroupTokens token tiles: within a group the token tiles
 // of one weight tile come one after another, so the CTAs at work at a time
 // share few weight tiles and few token tiles in L2.
-template <int BN>
-B200_DEVICE Tile tile_at(const LinearArgs& a, int tile) {
+// PAIR: a tile has twice the weight rows, and n0 is its second half in the
+// cluster's second CTA.
+template <int BN, bool PAIR>
+B200_DEVICE Tile tile_at(const LinearArgs& a, int tile, int rank) {
   const int per_group = kGroupTokens * a.n_tiles;
   const int g = tile / per_group;
   const int first = g * kGroupTokens;
@@ -169,7 +258,8 @@ B200_DEVICE Tile tile_at(const LinearArgs& a, int tile) {
   const int rem = tile - g * per_group;
   Tile t;
   t.token0 = (first + rem % rows) * BN;
-  t.n0 = rem / rows * (a.gated ? kRows / 2 : kRows);
+  const int n_tile = PAIR ? rem / rows * 2 + rank : rem / rows;
+  t.n0 = n_tile * (a.gated ? kRows / 2 : kRows);
   return t;
 }
 
@@ -290,14 +380,15 @@ struct Epilogue {
   }
 };
 
-template <int BN, bool FP8>
+template <int BN, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                   const LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers B;
   __shared__ __align__(16) float xs[kEpilogueWarps][32];  // token scales of a warp's columns
-  constexpr int kBBytes = BN * kKBytes;
+  constexpr int kBRows = PAIR ? BN / 2 : BN;  // tokens in this CTA's shared memory
+  constexpr int kBBytes = kBRows * kKBytes;
   constexpr int kStageBytes = kABytes + kBBytes;
   constexpr int kKElems = FP8 ? 128 : 64;
   constexpr uint32_t kTmemCols = 2 * BN;
@@ -319,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), kEpilogueThreads);
+      mbar_init(acc_empty(b), PAIR ? 2 * kEpilogueWarps : kEpilogueWarps);
     }
     B.error = 0;
     fence_mbar_init();
@@ -327,14 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&tm_x);
   }
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(&B.tmem_base)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc<PAIR>(smem_u32(&B.tmem_base), kTmemCols);
   }
   tc_fence_before();
-  if (a.splits > 1) cluster_sync();  // every CTA of the cluster runs before any writes to it
+  if (PAIR || a.splits > 1) cluster_sync();  // every CTA of the cluster runs before any writes to it
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = B.tmem_base;
@@ -343,36 +430,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool aborted = a.dev_status != nullptr &&
                        (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
 
-  const int rank = a.splits > 1 ? static_cast<int>(blockIdx.x) % a.splits : 0;
-  const int first = static_cast<int>(blockIdx.x) / a.splits;
-  const int stride = static_cast<int>(gridDim.x) / a.splits;
+  const int cluster = PAIR ? 2 : a.splits;
+  const int rank = static_cast<int>(blockIdx.x) % cluster;
+  const int first = static_cast<int>(blockIdx.x) / cluster;
+  const int stride = static_cast<int>(gridDim.x) / cluster;
   const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / a.splits);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / a.splits);
+  // PAIR: both CTAs work on all of K, for the first CTA's MMA lane
+  const int kb0 =
+      PAIR ? 0 : static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / a.splits);
+  const int kb1 = PAIR ? a.k_blocks
+                       : static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / a.splits);
 
   if (warp == kProducerWarp && lane == 0) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += stride) {
-      const Tile t = tile_at<BN>(a, tile);
+      const Tile t = tile_at<BN, PAIR>(a, tile, rank);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = wait_or_flag(empty(stage), phase ^ 1, &B, a.dev_status))) break;
-        const uint32_t bar = full(stage), dst = base + stage * kStageBytes;
+        // PAIR: both CTAs' copies count on the first CTA's barrier
+        const uint32_t bar = PAIR ? remote_smem(full(stage), 0) : full(stage);
+        const uint32_t dst = base + stage * kStageBytes;
         const int k0 = kb * kKElems;
-        mbar_arrive_expect_tx(bar, kStageBytes);
+        if (!PAIR || rank == 0) mbar_arrive_expect_tx(full(stage), (PAIR ? 2 : 1) * kStageBytes);
         if (a.gated == 2) {
-          tma_load_4d_nohint(dst, &tm_w, bar, k0, 0, 0, t.n0 / 16);
+          load_4d<PAIR>(dst, &tm_w, bar, k0, 0, 0, t.n0 / 16);
         } else if (a.gated == 1) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            tma_load_2d(dst + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
-            tma_load_2d(dst + g * 4096 + 2048, &tm_w, bar, k0, a.n + t.n0 + g * 16);
+            load_2d<PAIR>(dst + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
+            load_2d<PAIR>(dst + g * 4096 + 2048, &tm_w, bar, k0, a.n + t.n0 + g * 16);
           }
         } else {
-          tma_load_2d(dst, &tm_w, bar, k0, t.n0);
+          load_2d<PAIR>(dst, &tm_w, bar, k0, t.n0);
         }
-        tma_load_2d(dst + kABytes, &tm_x, bar, k0, t.token0);
+        load_2d<PAIR>(dst + kABytes, &tm_x, bar, k0, t.token0 + (PAIR ? rank * kBRows : 0));
         ++issued;
         if (++stage == a.stages) {
           stage = 0;
@@ -380,17 +473,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (!ok) {  // the copies in flight land before the CTA's shared memory goes away
+    // After a give-up the copies in flight land before the shared memory goes
+    // away (PAIR: the first CTA waits for both CTAs' copies, and the second stays
+    // until the cluster barrier at the end).
+    if (!ok && (!PAIR || rank == 0)) {
       for (int i = 0; i < min(issued, a.stages); ++i) {
         if (--stage < 0) {
           stage = a.stages - 1;
           phase ^= 1;
         }
-        mbar_wait_bounded(full(stage), phase);
+        mbar_wait_abortable(full(stage), phase, nullptr, kDrainLimitNs);
       }
     }
-  } else if (warp == kMmaWarp && lane == 0) {
-    constexpr uint32_t idesc = instruction<FP8>(BN);
+  } else if (warp == kMmaWarp && lane == 0 && (!PAIR || rank == 0)) {
+    constexpr uint32_t idesc = instruction<FP8>(PAIR ? 2 * kRows : kRows, BN);
     int stage = 0, count = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -404,22 +500,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t sa = base + stage * kStageBytes, sb = sa + kABytes;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          mma<FP8>(tmem + buf * BN, smem_desc(sa + j * 32, 16, 1024), smem_desc(sb + j * 32, 16, 1024),
-                   idesc, kb > kb0 || j > 0 ? 1u : 0u);
-        umma_commit(empty(stage));
+          mma<FP8, PAIR>(tmem + buf * BN, smem_desc(sa + j * 32, 16, 1024),
+                         smem_desc(sb + j * 32, 16, 1024), idesc, kb > kb0 || j > 0 ? 1u : 0u);
+        commit<PAIR>(empty(stage));
         if (++stage == a.stages) {
           stage = 0;
           phase ^= 1;
         }
       }
-      if (ok) umma_commit(acc_full(buf));
+      if (ok) commit<PAIR>(acc_full(buf));
     }
   } else if (warp < kEpilogueWarps) {
     const int part = warp >> 2;  // which of every two 32-column groups
     const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
-      const Tile t = tile_at<BN>(a, tile);
+      const Tile t = tile_at<BN, PAIR>(a, tile, rank);
       const int buf = count & 1;
       const uint32_t acc = tmem + lane0 + buf * BN;
       const Epilogue ep(a, t.n0, warp, lane);
@@ -442,7 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                              [&] { tmem_wait_ld(reinterpret_cast<uint32_t*>(v)); });
         }
         tc_fence_before();
-        mbar_arrive(acc_empty(buf));
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) arrive_remote(remote_smem(acc_empty(buf), 0));
+          else mbar_arrive(acc_empty(buf));
+        }
       } else {
         // column c belongs to rank c / own: into that CTA's exchange buffer
         const int own = BN / a.splits, shift = __ffs(own) - 1;
@@ -463,10 +563,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   __syncwarp();
-  if (a.splits > 1) {  // one tile a cluster
+  if (!PAIR && a.splits > 1) {  // one tile a cluster
     cluster_sync();
     if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
-      const Tile t = tile_at<BN>(a, first);
+      const Tile t = tile_at<BN, PAIR>(a, first, rank);
       const Epilogue ep(a, t.n0, warp, lane);
       const int own = BN / a.splits;
       const int token0 = t.token0 + rank * own;
@@ -488,13 +588,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA is done with this one's barriers and TMEM
+  else __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(kTmemCols)
-                 : "memory");
-  }
+  if (warp == kMmaWarp) tmem_dealloc<PAIR>(tmem, kTmemCols);
 }
 
 // ------------------------------------------------------------------ host side
@@ -502,10 +599,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 std::mutex g_attr_mu;
 bool g_attr_done[64] = {false};
 
-template <int BN, bool FP8>
+template <int BN, bool FP8, bool PAIR>
 cudaError_t set_smem_attr() {
-  return cudaFuncSetAttribute(linear_kernel<BN, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              kSmemBudget + 1024);
+  return cudaFuncSetAttribute(linear_kernel<BN, FP8, PAIR>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget + 1024);
+}
+
+template <bool FP8>
+cudaError_t set_smem_attrs() {
+  const cudaError_t es[] = {set_smem_attr<32, FP8, false>(), set_smem_attr<64, FP8, false>(),
+                            set_smem_attr<128, FP8, false>(), set_smem_attr<256, FP8, false>(),
+                            set_smem_attr<256, FP8, true>()};
+  for (cudaError_t e : es)
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
 }
 
 int ensure_smem_attr(int dev) {
@@ -513,12 +620,9 @@ int ensure_smem_attr(int dev) {
   if (dev < 64 && g_attr_done[dev]) return B200_OK;
   std::lock_guard<std::mutex> lk(g_attr_mu);
   if (dev < 64 && g_attr_done[dev]) return B200_OK;
-  const cudaError_t es[] = {set_smem_attr<32, false>(),  set_smem_attr<64, false>(),
-                            set_smem_attr<128, false>(), set_smem_attr<256, false>(),
-                            set_smem_attr<32, true>(),   set_smem_attr<64, true>(),
-                            set_smem_attr<128, true>(),  set_smem_attr<256, true>()};
-  for (cudaError_t e : es)
-    if (e != cudaSuccess) return b200host::status_from_cuda(e);
+  cudaError_t e = set_smem_attrs<false>();
+  if (e == cudaSuccess) e = set_smem_attrs<true>();
+  if (e != cudaSuccess) return b200host::status_from_cuda(e);
   if (dev < 64) g_attr_done[dev] = true;
   return B200_OK;
 }
@@ -557,16 +661,18 @@ int encode_gated(CUtensorMap* map, const void* base, int64_t n, int64_t k, int64
              : B200_ERR_TENSOR_MAP;
 }
 
-template <int BN, bool FP8>
+template <int BN, bool FP8, bool PAIR>
 cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, int sms,
                    cudaStream_t stream) {
-  const int stage_bytes = kABytes + BN * kKBytes;
+  const int stage_bytes = kABytes + (PAIR ? BN / 2 : BN) * kKBytes;
   const int exchange = a.splits > 1 ? BN * kRows * 4 : 0;
   a.stages = (kSmemBudget - exchange) / stage_bytes;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
-  const int grid = a.splits > 1 ? static_cast<int>(tiles) * a.splits
-                                : static_cast<int>(tiles < sms ? tiles : sms);
+  const int cluster = PAIR ? 2 : a.splits;
+  const int64_t ctas = static_cast<int64_t>(a.m_tiles) * a.n_tiles * cluster;
+  // without a split of K the CTAs (or pairs) persist and take tiles in turn
+  const int resident = sms / cluster * cluster;
+  const int grid = static_cast<int>(a.splits > 1 || ctas < resident ? ctas : resident);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
@@ -576,22 +682,23 @@ cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, i
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(a.splits);
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, linear_kernel<BN, FP8>, tw, tx, a);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, linear_kernel<BN, FP8, PAIR>, tw, tx, a);
 }
 
 template <bool FP8>
-cudaError_t launch_bn(int bn, const CUtensorMap& tw, const CUtensorMap& tx, const LinearArgs& a,
-                      int sms, cudaStream_t stream) {
+cudaError_t launch_bn(int bn, bool pair, const CUtensorMap& tw, const CUtensorMap& tx,
+                      const LinearArgs& a, int sms, cudaStream_t stream) {
+  if (pair) return launch<256, FP8, true>(tw, tx, a, sms, stream);
   switch (bn) {
-    case 32: return launch<32, FP8>(tw, tx, a, sms, stream);
-    case 64: return launch<64, FP8>(tw, tx, a, sms, stream);
-    case 128: return launch<128, FP8>(tw, tx, a, sms, stream);
-    default: return launch<256, FP8>(tw, tx, a, sms, stream);
+    case 32: return launch<32, FP8, false>(tw, tx, a, sms, stream);
+    case 64: return launch<64, FP8, false>(tw, tx, a, sms, stream);
+    case 128: return launch<128, FP8, false>(tw, tx, a, sms, stream);
+    default: return launch<256, FP8, false>(tw, tx, a, sms, stream);
   }
 }
 
@@ -642,12 +749,14 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   a.n_tiles = (n + tile_n - 1) / tile_n;
   const int bn = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
   a.m_tiles = (m + bn - 1) / bn;
-  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
+  int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
   if (tiles > 0x3fffffff) return B200_ERR_INVALID_ARGUMENT;
   a.splits = 1;
   if (bn <= 64)
     while (a.splits < kMaxSplits && tiles * a.splits * 2 <= sms && a.splits * 4 <= a.k_blocks)
       a.splits *= 2;
+  const bool pair = bn == 256 && tiles >= sms;
+  if (pair) a.n_tiles = (a.n_tiles + 1) / 2;
 
   CUtensorMap tw, tx;
   if (a.gated == 2)
@@ -655,9 +764,9 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   else
     st = encode_rows(&tw, w, gated ? 2 * static_cast<int64_t>(n) : n, k, w_stride, fp8 != 0,
                      gated ? 16 : kRows);
-  if (st == B200_OK) st = encode_rows(&tx, x, m, k, x_stride, fp8 != 0, bn);
+  if (st == B200_OK) st = encode_rows(&tx, x, m, k, x_stride, fp8 != 0, pair ? bn / 2 : bn);
   if (st != B200_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, tw, tx, a, sms, cs)
-                                        : launch_bn<false>(bn, tw, tx, a, sms, cs));
+  return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, pair, tw, tx, a, sms, cs)
+                                        : launch_bn<false>(bn, pair, tw, tx, a, sms, cs));
 }

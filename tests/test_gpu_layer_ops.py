@@ -220,7 +220,9 @@ def _check_product(got, a, act, gated):
 PRODUCT_SIZES = [(1, 8, 1), (1, 64, 128), (1, 1000, 257), (2, 16, 3), (5, 1024, 384), (8, 1024, 4096),
                  (31, 136, 100), (33, 200, 129), (64, 4096, 1024), (65, 512, 640), (127, 768, 96),
                  (129, 320, 130), (200, 1001, 77), (257, 264, 1000), (300, 2048, 2050), (1, 12288, 16),
-                 (17, 20000, 65), (511, 65, 511)]
+                 (17, 20000, 65), (511, 65, 511),
+                 # enough tiles for pairs of CTAs: an odd number of weight tiles, ragged ends
+                 (257, 128, 9500), (600, 192, 6400), (1000, 72, 4999), (2049, 1024, 2048)]
 
 
 @pytest.mark.parametrize("m,k,n", PRODUCT_SIZES)
