@@ -307,22 +307,29 @@ struct Epilogue {
   B200_DEVICE void put_all(int token, int step, const float (&v)[N],
                            const uint32_t (&res)[N / 2], bool fast) const {
     const int first = token + (odd ? step : 0);
-    __nv_bfloat16* o = a.out + first * a.o_row + pair_n;
-    const int64_t jump = 2 * step * a.o_row;
+    float lo[N / 2], hi[N / 2];
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
-      float lo = odd ? got : v[i], hi = odd ? v[i + 1] : got;
-      if (fast) {
-        if (a.residual != nullptr) {
-          lo += bf16_lo(res[i / 2]);
-          hi += bf16_hi(res[i / 2]);
+    for (int i = 0; i < N / 2; ++i) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
+      lo[i] = odd ? got : v[2 * i];
+      hi[i] = odd ? v[2 * i + 1] : got;
+    }
+    if (fast) {
+      if (a.residual != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          lo[i] += bf16_lo(res[i]);
+          hi[i] += bf16_hi(res[i]);
         }
-        *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(lo, hi);
-        o += jump;
-      } else {
-        put(first + i * step, lo, hi);
       }
+      __nv_bfloat16* o = a.out + first * a.o_row + pair_n;
+      const int64_t jump = 2 * step * a.o_row;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        *reinterpret_cast<uint32_t*>(o + i * jump) = pack_bf16x2(lo[i], hi[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) put(first + 2 * i * step, lo[i], hi[i]);
     }
   }
 
@@ -386,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers B;
-  __shared__ __align__(16) float xs[kEpilogueWarps][32];  // token scales of a warp's columns
+  __shared__ __align__(16) float xs[kEpilogueWarps][128];  // token scales of a warp's columns
   constexpr int kBRows = PAIR ? BN / 2 : BN;  // tokens in this CTA's shared memory
   constexpr int kBBytes = kBRows * kKBytes;
   constexpr int kStageBytes = kABytes + kBBytes;
@@ -410,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), PAIR ? 2 * kEpilogueWarps : kEpilogueWarps);
+      // PAIR: the first CTA's MMA lane also hears from the second CTA
+      mbar_init(acc_empty(b), kEpilogueWarps + (PAIR && blockIdx.x % 2 == 0 ? 1 : 0));
     }
     B.error = 0;
     fence_mbar_init();
@@ -510,6 +518,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) commit<PAIR>(acc_full(buf));
     }
+  } else if (PAIR && warp == kMmaWarp && lane == 0) {
+    // Second CTA: passes on that its accumulators were read.  From here, not from
+    // the epilogue: a release to the cluster waits for the thread's stores.
+    int count = 0;
+    for (int tile = first; tile < tiles; tile += stride, ++count) {
+      const int buf = count & 1;
+      if (!wait_or_flag(acc_empty(buf), (count >> 1) & 1, &B, a.dev_status)) break;
+      arrive_remote(remote_smem(acc_empty(buf), 0));
+    }
   } else if (warp < kEpilogueWarps) {
     const int part = warp >> 2;  // which of every two 32-column groups
     const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -519,30 +536,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int buf = count & 1;
       const uint32_t acc = tmem + lane0 + buf * BN;
       const Epilogue ep(a, t.n0, warp, lane);
+      constexpr int kGroups = (BN + 63) / 64;  // 32-column groups of this warp
+      const int cols = min(BN, a.m - t.token0);
+      if (a.w_scale != nullptr && a.splits == 1) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          const int c = part * 32 + j * 64 + lane;
+          xs[warp][j * 32 + lane] = c < cols ? a.x_scale[t.token0 + c] : 0.0f;
+        }
+        __syncwarp();
+      }
       bool ok = wait_or_flag(acc_full(buf), (count >> 1) & 1, &B, a.dev_status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       if (a.splits == 1) {
-        const int cols = min(BN, a.m - t.token0);
 #pragma unroll 1
-        for (int c = part * 32; c < cols; c += 64) {
+        for (int c = part * 32, j = 0; c < cols; c += 64, j += 32) {
           float v[32];
           tmem_ld32(acc + c, reinterpret_cast<uint32_t*>(v));
-          if (a.w_scale != nullptr) {
-            __syncwarp();
-            xs[warp][lane] = c + lane < cols ? a.x_scale[t.token0 + c + lane] : 0.0f;
-            __syncwarp();
-          }
-          ep.put_columns<32>(t.token0 + c, v, xs[warp],
+          ep.put_columns<32>(t.token0 + c, v, &xs[warp][j],
                              [&] { tmem_wait_ld(reinterpret_cast<uint32_t*>(v)); });
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (PAIR) arrive_remote(remote_smem(acc_empty(buf), 0));
-          else mbar_arrive(acc_empty(buf));
-        }
+        if (lane == 0) mbar_arrive(acc_empty(buf));
       } else {
         // column c belongs to rank c / own: into that CTA's exchange buffer
         const int own = BN / a.splits, shift = __ffs(own) - 1;
