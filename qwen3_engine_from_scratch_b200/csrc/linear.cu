@@ -46,7 +46,6 @@ constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kMaxStages = 10;
 constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
-constexpr int kMaxSplits = 8;
 constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s a pipeline wait
 constexpr uint64_t kDrainLimitNs = 100000000ull;   // 0.1 s a copy after a give-up
@@ -617,6 +616,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 std::mutex g_attr_mu;
 bool g_attr_done[64] = {false};
+// CTAs of clusters of 1, 2, 4 and 8 that a device holds at once (clusters do not
+// span its GPCs: 8 CTAs a cluster leave some SMs without one)
+int g_resident[64][4];
 
 template <int BN, bool FP8, bool PAIR>
 cudaError_t set_smem_attr() {
@@ -635,15 +637,77 @@ cudaError_t set_smem_attrs() {
 }
 
 int ensure_smem_attr(int dev) {
-  if (dev < 0) return B200_ERR_CUDA;
-  if (dev < 64 && g_attr_done[dev]) return B200_OK;
+  if (dev < 0 || dev >= 64) return B200_ERR_CUDA;
+  if (g_attr_done[dev]) return B200_OK;
   std::lock_guard<std::mutex> lk(g_attr_mu);
-  if (dev < 64 && g_attr_done[dev]) return B200_OK;
+  if (g_attr_done[dev]) return B200_OK;
   cudaError_t e = set_smem_attrs<false>();
   if (e == cudaSuccess) e = set_smem_attrs<true>();
   if (e != cudaSuccess) return b200host::status_from_cuda(e);
-  if (dev < 64) g_attr_done[dev] = true;
+  g_resident[dev][0] = b200host::sm_count(dev);
+  for (int i = 1; i < 4; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << i);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBudget;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << i;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    e = cudaOccupancyMaxActiveClusters(&clusters, linear_kernel<32, false, false>, &cfg);
+    if (e != cudaSuccess) return b200host::status_from_cuda(e);
+    g_resident[dev][i] = clusters << i;
+  }
+  g_attr_done[dev] = true;
   return B200_OK;
+}
+
+// How a product is cut: token tiles of bn, CTAs of a cluster that split K, or
+// pairs of CTAs with 256 x 256 tiles.
+struct Plan {
+  int bn, splits;
+  bool pair;
+};
+
+// The cut with the least estimated time, from a model of measured launches
+// (us): 4 for a launch and its first loads; a stage of 128 bytes of K costs 0.26
+// to 0.40 with the tile's width (64 bytes a clock into an SM, then the MMAs);
+// the last tile's epilogue and, where K is split, the exchange are in the open.
+// It gives the measured best or comes within 10 % of it over 18 shapes from 1 to
+// 2048 tokens: 128 x 4096 x 4096 takes 14.5 us with K split 4 ways (bn 128)
+// and 22.6 without, 512 x 4096 x 4096 24.1 with bn 128 and 26.6 with 256,
+// 1024 x 4096 x 4096 27.7 in pairs and 43.9 with bn 128.
+Plan choose(int m, int n_tiles, int k_blocks, const int* resident) {
+  constexpr int kBn[] = {32, 64, 128, 256, 256};
+  constexpr float kStage[] = {0.26f, 0.28f, 0.31f, 0.40f, 0.36f};
+  constexpr float kEpilogue[] = {0.5f, 0.7f, 1.2f, 2.2f, 2.2f};
+  constexpr float kExchange[] = {0.8f, 1.2f, 3.7f};
+  Plan best{32, 1, false};
+  float least = 3.4e38f;
+  for (int i = 0; i < 5; ++i) {
+    const bool pair = i == 4;
+    const int64_t tiles = static_cast<int64_t>((m + kBn[i] - 1) / kBn[i]) *
+                          (pair ? (n_tiles + 1) / 2 : n_tiles);
+    for (int log = 0; log < (i < 3 ? 4 : 1); ++log) {
+      const int splits = 1 << log;
+      if (splits > 1 && splits * 2 > k_blocks) break;
+      const int64_t room = pair ? resident[1] / 2 : resident[log] / splits;
+      if (room == 0) continue;
+      const float waves = static_cast<float>((tiles + room - 1) / room);
+      if (splits > 1 && waves > 1.0f) break;  // clusters that split K do not persist
+      const float t = 4.0f + waves * ((k_blocks + splits - 1) / splits) * kStage[i] + kEpilogue[i] +
+                      (splits > 1 ? kExchange[i] : 0.0f);
+      if (t < least) {
+        least = t;
+        best = Plan{kBn[i], splits, pair};
+      }
+    }
+  }
+  return best;
 }
 
 // rows x k elements of `size` bytes, K innermost
@@ -690,7 +754,7 @@ cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, i
   const int cluster = PAIR ? 2 : a.splits;
   const int64_t ctas = static_cast<int64_t>(a.m_tiles) * a.n_tiles * cluster;
   // without a split of K the CTAs (or pairs) persist and take tiles in turn
-  const int resident = sms / cluster * cluster;
+  const int resident = PAIR ? g_resident[b200host::current_device()][1] : sms;
   const int grid = static_cast<int>(a.splits > 1 || ctas < resident ? ctas : resident);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
@@ -766,16 +830,13 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
 
   const int tile_n = gated ? kRows / 2 : kRows;
   a.n_tiles = (n + tile_n - 1) / tile_n;
-  const int bn = m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+  const Plan plan = choose(m, a.n_tiles, a.k_blocks, g_resident[dev]);
+  const int bn = plan.bn;
+  const bool pair = plan.pair;
   a.m_tiles = (m + bn - 1) / bn;
-  int64_t tiles = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
-  if (tiles > 0x3fffffff) return B200_ERR_INVALID_ARGUMENT;
-  a.splits = 1;
-  if (bn <= 64)
-    while (a.splits < kMaxSplits && tiles * a.splits * 2 <= sms && a.splits * 4 <= a.k_blocks)
-      a.splits *= 2;
-  const bool pair = bn == 256 && tiles >= sms;
+  a.splits = plan.splits;
   if (pair) a.n_tiles = (a.n_tiles + 1) / 2;
+  if (static_cast<int64_t>(a.m_tiles) * a.n_tiles > 0x0fffffff) return B200_ERR_INVALID_ARGUMENT;
 
   CUtensorMap tw, tx;
   if (a.gated == 2)
