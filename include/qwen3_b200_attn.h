@@ -402,7 +402,7 @@ int b200_qk_norm_rope_kv_write(
 int b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
                   const void* weight, void* y, int64_t y_stride, float* scale,
                   void* residual_out, int64_t h_stride, int64_t rows, int hidden, float eps,
-                  void* stream);
+                  int32_t* dev_status, void* stream);
 
 /* Activations of b200_linear. */
 #define B200_ACT_NONE 0

@@ -90,7 +90,7 @@ SIGNATURES = {
                                         _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                         _P, _P, _I64, _P,
                                         _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
-    "b200_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I, _F, _P]),
+    "b200_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I, _F, _P, _P]),
     "b200_linear": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64,
                          _I, _I, _I, _I, _I, _I, _P, _P]),
     "b200_rotary": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64,

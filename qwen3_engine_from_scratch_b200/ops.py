@@ -918,7 +918,7 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
         assert residual_out is None, "residual_out needs a residual"
     st = _native.load().b200_rms_norm(x2.data_ptr(), x2.stride(0), r_ptr, r_stride, w_ptr,
                                       y.data_ptr(), y_stride, s_ptr, h_ptr, h_stride, rows, hidden,
-                                      eps, _stream_of(index))
+                                      eps, _status_ptr(x.device), _stream_of(index))
     if st:
         _native.check(st, what)
     if fp8:

@@ -56,7 +56,9 @@ def _place(t, how):
 # ---------------------------------------------------------------- norm
 
 NORM_SIZES = [(1, 1), (1, 7), (3, 8), (5, 31), (2, 32), (300, 128), (7, 1000), (9, 1024),
-              (4, 1537), (65, 2048), (3, 4096), (2, 8200), (2, 9001), (2, 12288), (2, 32776)]
+              (4, 1537), (65, 2048), (3, 4096), (2, 8200), (2, 9001), (2, 12288), (2, 32776),
+              # many wide rows: the streaming form, every number of CTAs an SM
+              (700, 2048), (1300, 4104), (700, 5120), (640, 8192), (3001, 12288), (640, 16384)]
 
 
 def _norm_exact(x, w, r, eps):
@@ -110,24 +112,26 @@ def test_norm_in_place_and_batched(qb):
     assert torch.equal(x2, want[0]) and torch.equal(r2, want[1])
     q, s, _ = qb.rms_norm_fp8(x, w, residual=r)
     assert q.shape == x.shape and s.shape == (2, 5)
-    # wide rows that are read twice, in place
-    x, r = _randn(g, 2, 40000).to(BF16), _randn(g, 2, 40000).to(BF16)
-    w = torch.ones(40000, dtype=BF16, device="cuda")
-    want, h = _norm_exact(x, w, r, 1e-6)
-    y, h2 = qb.rms_norm(x, w, residual=r, residual_out=r)
-    _check_bf16(y, want)
-    _check_bf16(h2, h)
+    # wide rows that are read twice, and streamed ones, in place
+    for rows, hidden in ((2, 40000), (1000, 4096)):
+        x, r = _randn(g, rows, hidden).to(BF16), _randn(g, rows, hidden).to(BF16)
+        w = torch.ones(hidden, dtype=BF16, device="cuda")
+        want, h = _norm_exact(x, w, r, 1e-6)
+        y, h2 = qb.rms_norm(x, w, residual=r, residual_out=r)
+        _check_bf16(y, want)
+        _check_bf16(h2, h)
 
 
 def test_norm_special_rows(qb):
     """Zero rows, NaN and infinities: what the definition gives, row by row."""
-    x = _randn(_gen(5), 6, 520).to(BF16)
-    x[1] = 0
-    x[2, 17] = float("nan")
-    x[3, 519] = float("inf")
-    x[4] *= 1e-30
-    w = torch.ones(520, dtype=BF16, device="cuda")
-    for size in (520, 519):          # vectors and single elements
+    for rows, wide, size in ((6, 520, 520), (6, 520, 519), (800, 4096, 4096)):
+        # vectors, single elements, streamed rows
+        x = _randn(_gen(5), rows, wide).to(BF16)
+        x[1] = 0
+        x[2, 17] = float("nan")
+        x[3, wide - 1] = float("inf")
+        x[4] *= 1e-30
+        w = torch.ones(wide, dtype=BF16, device="cuda")
         xs, ws = x[:, -size:], w[-size:]
         y = qb.rms_norm(xs, ws)
         want, _ = _norm_exact(xs, ws, None, 1e-6)

@@ -65,7 +65,8 @@ def test_c_entry_refusals(native_lib):
     lib = native_lib
     fake, odd = 16, 18
     norm = lambda **k: lib.b200_rms_norm(*{**dict(x=fake, xs=8, r=None, rs=0, w=fake, y=fake, ys=8, s=None,  # noqa: E731
-                                                  h=None, hs=0, rows=1, hidden=8, eps=1e-6, st=None), **k}.values())
+                                                  h=None, hs=0, rows=1, hidden=8, eps=1e-6, dev=None,
+                                                  st=None), **k}.values())
     assert norm(rows=0) == 0
     assert norm(rows=-1) == -1 and norm(hidden=0) == -1 and norm(x=None) == -1
     assert norm(r=fake) == -1 and norm(h=fake) == -1 and norm(w=None) == -1
