@@ -10,10 +10,10 @@
 // bits then go through sincospi.  A product in fp32 would lose position * 2^-24
 // radians: 0.008 at position 131,072.
 //
-// Bound by memory for prefills: q and k are read and written once.  A thread
-// takes one slot of 16 elements (8 pairs, or 16 copied elements) of one token
-// and walks over some of the token's heads, so its 8 sines and cosines are
-// computed once for several heads.
+// Bound by memory for prefills: q and k are read and written once.  A block
+// takes a few tokens: it computes their sines and cosines once into shared
+// memory, then its threads (16 elements of a head each: 8 pairs, or 16 copied
+// elements; neighbours in a head, then in heads) walk over the tokens' heads.
 #include "common.cuh"
 
 namespace {
@@ -30,10 +30,12 @@ struct RotaryArgs {
   int heads_q, heads;           // q heads, q + k heads
   int seq;                      // tokens of a sequence
   int dim, rotary_dim;
-  int slots;                    // slots of a head
-  int groups;                   // threads that share a (token, slot), each with some heads
+  int slots;                    // slots of a head: 16 elements, or one pair / element
+  int slot_threads;             // threads of a head (a divisor of the block with the next two)
+  int groups;                   // heads at work at a time
+  int block_tokens;
   int interleaved;
-  int64_t work;                 // threads with work
+  int64_t tokens;
 };
 
 B200_DEVICE void angle(const uint64_t* turns, int i, int64_t position, float gain, float& c,
@@ -47,106 +49,147 @@ B200_DEVICE void angle(const uint64_t* turns, int i, int64_t position, float gai
   s *= gain;
 }
 
+struct Place {
+  int64_t b, s;
+};
+B200_DEVICE Place place_of(const RotaryArgs& a, int64_t token) {
+  Place p{0, token};
+  if (a.tokens > a.seq) {  // several sequences
+    if (a.tokens <= 0x7fffffff) {
+      p.b = static_cast<uint32_t>(token) / static_cast<uint32_t>(a.seq);
+      p.s = static_cast<uint32_t>(token) % static_cast<uint32_t>(a.seq);
+    } else {
+      p.b = token / a.seq;
+      p.s = token - p.b * a.seq;
+    }
+  }
+  return p;
+}
+
 B200_DEVICE int64_t position_of(const RotaryArgs& a, int64_t token) {
-  const int64_t b = token / a.seq, s = token - b * a.seq;
-  const int64_t at = b * a.pos_b + s * a.pos_s;
+  const Place p = place_of(a, token);
+  const int64_t at = p.b * a.pos_b + p.s * a.pos_s;
   return a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
                  : static_cast<const int32_t*>(a.positions)[at];
 }
 
-// first element of a token's head in q or k (`which`)
-B200_DEVICE const __nv_bfloat16* head_in(const RotaryArgs& a, int64_t b, int64_t s, int head,
-                                         int& which) {
-  which = head >= a.heads_q;
-  const int h = which ? head - a.heads_q : head;
-  return which ? a.in[1] + b * a.in_b[1] + h * a.in_h[1] + s * a.in_s[1]
-               : a.in[0] + b * a.in_b[0] + h * a.in_h[0] + s * a.in_s[0];
-}
-B200_DEVICE __nv_bfloat16* head_out(const RotaryArgs& a, int64_t b, int64_t s, int head) {
-  const int which = head >= a.heads_q;
-  const int h = which ? head - a.heads_q : head;
-  return which ? a.out[1] + b * a.out_b[1] + h * a.out_h[1] + s * a.out_s[1]
-               : a.out[0] + b * a.out_b[0] + h * a.out_h[0] + s * a.out_s[0];
-}
-
-// Slots of 16 elements, moved as two 16-byte vectors.
-__global__ void __launch_bounds__(256) rotary_vector_kernel(const RotaryArgs a) {
+// VEC: slots of 16 elements moved as two 16-byte vectors; otherwise any size,
+// stride and alignment, and a slot is one pair or one copied element.
+// Two heads ahead of a thread and three blocks an SM: 16,384 tokens of 32 + 8
+// heads of 128 in 57.6 us (5.8 TB/s, 0.89 of the copy rate) with half of the head
+// turning, 59.6 with all of it.  One head ahead: 61 to 66 us; four heads and two
+// blocks, 62.8.
+template <bool VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ float2 turn[];  // [token of the block][pair]: cos, sin
   b200::pdl_begin();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= a.work) return;
-  const int slot = static_cast<int>(i % a.slots);
-  const int64_t rest = i / a.slots;
-  const int group = static_cast<int>(rest % a.groups);
-  const int64_t token = rest / a.groups;
-  const int64_t b = token / a.seq, s = token - b * a.seq;
-  const bool turn = slot * 16 < a.rotary_dim;
-  const bool split = turn && !a.interleaved;
-  const int e0 = split ? slot * 8 : slot * 16;
-  const int e1 = split ? e0 + a.rotary_dim / 2 : e0 + 8;
-
-  float c[8], sn[8];
-  if (turn) {
-    const int64_t position = position_of(a, token);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) angle(a.turns, slot * 8 + j, position, a.gain, c[j], sn[j]);
-  }
-  for (int head = group; head < a.heads; head += a.groups) {
-    int which;
-    const __nv_bfloat16* in = head_in(a, b, s, head, which);
-    __nv_bfloat16* out = head_out(a, b, s, head);
-    const uint4 u0 = *reinterpret_cast<const uint4*>(in + e0);
-    const uint4 u1 = *reinterpret_cast<const uint4*>(in + e1);
-    uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
-    if (split) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a0 = b200::bf16_lo(w0[j]), a1 = b200::bf16_hi(w0[j]);
-        const float b0 = b200::bf16_lo(w1[j]), b1 = b200::bf16_hi(w1[j]);
-        w0[j] = b200::pack_bf16x2(a0 * c[2 * j] - b0 * sn[2 * j],
-                                  a1 * c[2 * j + 1] - b1 * sn[2 * j + 1]);
-        w1[j] = b200::pack_bf16x2(b0 * c[2 * j] + a0 * sn[2 * j],
-                                  b1 * c[2 * j + 1] + a1 * sn[2 * j + 1]);
-      }
-    } else if (turn) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a0 = b200::bf16_lo(w0[j]), b0 = b200::bf16_hi(w0[j]);
-        const float a1 = b200::bf16_lo(w1[j]), b1 = b200::bf16_hi(w1[j]);
-        w0[j] = b200::pack_bf16x2(a0 * c[j] - b0 * sn[j], b0 * c[j] + a0 * sn[j]);
-        w1[j] = b200::pack_bf16x2(a1 * c[4 + j] - b1 * sn[4 + j], b1 * c[4 + j] + a1 * sn[4 + j]);
-      }
-    }
-    *reinterpret_cast<uint4*>(out + e0) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
-    *reinterpret_cast<uint4*>(out + e1) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
-  }
-}
-
-// Any size, stride and alignment: a slot is one pair, or one copied element.
-__global__ void __launch_bounds__(256) rotary_scalar_kernel(const RotaryArgs a) {
-  b200::pdl_begin();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= a.work) return;
-  const int slot = static_cast<int>(i % a.slots);
-  const int64_t rest = i / a.slots;
-  const int group = static_cast<int>(rest % a.groups);
-  const int64_t token = rest / a.groups;
-  const int64_t b = token / a.seq, s = token - b * a.seq;
   const int half = a.rotary_dim / 2;
-  const bool turn = slot < half;
-  const int e0 = !turn ? half + slot : a.interleaved ? 2 * slot : slot;
-  const int e1 = a.interleaved ? e0 + 1 : e0 + half;
-  float c = 1.0f, sn = 0.0f;
-  if (turn) angle(a.turns, slot, position_of(a, token), a.gain, c, sn);
-  for (int head = group; head < a.heads; head += a.groups) {
-    int which;
-    const __nv_bfloat16* in = head_in(a, b, s, head, which);
-    __nv_bfloat16* out = head_out(a, b, s, head);
-    if (turn) {
-      const float x = __bfloat162float(in[e0]), y = __bfloat162float(in[e1]);
-      out[e0] = __float2bfloat16_rn(x * c - y * sn);
-      out[e1] = __float2bfloat16_rn(y * c + x * sn);
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * a.block_tokens;
+  const int block_tokens =
+      static_cast<int>(a.tokens - token0 < a.block_tokens ? a.tokens - token0 : a.block_tokens);
+  for (int i = threadIdx.x; i < block_tokens * half; i += blockDim.x) {
+    const int t = i / half;
+    float2 v;
+    angle(a.turns, i - t * half, position_of(a, token0 + t), a.gain, v.x, v.y);
+    turn[i] = v;
+  }
+  __syncthreads();
+  int rest = threadIdx.x / a.slot_threads;
+  const int slot0 = threadIdx.x - rest * a.slot_threads;
+  const int t = rest / a.groups;
+  const int group = rest - t * a.groups;
+  if (t >= block_tokens) return;
+  const Place p = place_of(a, token0 + t);
+  // where the token lies in q and k, in and out
+  const __nv_bfloat16* in_q = a.in[0] + p.b * a.in_b[0] + p.s * a.in_s[0];
+  const __nv_bfloat16* in_k = a.in[1] + p.b * a.in_b[1] + p.s * a.in_s[1];
+  __nv_bfloat16* out_q = a.out[0] + p.b * a.out_b[0] + p.s * a.out_s[0];
+  __nv_bfloat16* out_k = a.out[1] + p.b * a.out_b[1] + p.s * a.out_s[1];
+  auto in_at = [&](int head) {
+    return head < a.heads_q ? in_q + head * a.in_h[0] : in_k + (head - a.heads_q) * a.in_h[1];
+  };
+  auto out_at = [&](int head) {
+    return head < a.heads_q ? out_q + head * a.out_h[0] : out_k + (head - a.heads_q) * a.out_h[1];
+  };
+
+  for (int slot = slot0; slot < a.slots; slot += a.slot_threads) {
+    if constexpr (VEC) {
+      const bool turns = slot * 16 < a.rotary_dim;
+      const bool split = turns && !INTERLEAVED;
+      const int e0 = split ? slot * 8 : slot * 16;
+      const int e1 = split ? e0 + half : e0 + 8;
+      float c[8], sn[8];
+      if (turns) {
+        const float4* from = reinterpret_cast<const float4*>(turn + t * half + slot * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 v = from[j];
+          c[2 * j] = v.x;
+          sn[2 * j] = v.y;
+          c[2 * j + 1] = v.z;
+          sn[2 * j + 1] = v.w;
+        }
+      }
+      // kAhead heads are read before the first of them is written
+      constexpr int kAhead = 2;
+      for (int first = group; first < a.heads; first += kAhead * a.groups) {
+        uint4 u[kAhead][2];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int head = first + i * a.groups;
+          if (head < a.heads) {
+            const __nv_bfloat16* in = in_at(head);
+            u[i][0] = *reinterpret_cast<const uint4*>(in + e0);
+            u[i][1] = *reinterpret_cast<const uint4*>(in + e1);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int head = first + i * a.groups;
+          if (head >= a.heads) break;
+          uint32_t w0[4] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w};
+          uint32_t w1[4] = {u[i][1].x, u[i][1].y, u[i][1].z, u[i][1].w};
+          if (split) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float a0 = b200::bf16_lo(w0[j]), a1 = b200::bf16_hi(w0[j]);
+              const float b0 = b200::bf16_lo(w1[j]), b1 = b200::bf16_hi(w1[j]);
+              w0[j] = b200::pack_bf16x2(a0 * c[2 * j] - b0 * sn[2 * j],
+                                        a1 * c[2 * j + 1] - b1 * sn[2 * j + 1]);
+              w1[j] = b200::pack_bf16x2(b0 * c[2 * j] + a0 * sn[2 * j],
+                                        b1 * c[2 * j + 1] + a1 * sn[2 * j + 1]);
+            }
+          } else if (turns) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float a0 = b200::bf16_lo(w0[j]), b0 = b200::bf16_hi(w0[j]);
+              const float a1 = b200::bf16_lo(w1[j]), b1 = b200::bf16_hi(w1[j]);
+              w0[j] = b200::pack_bf16x2(a0 * c[j] - b0 * sn[j], b0 * c[j] + a0 * sn[j]);
+              w1[j] = b200::pack_bf16x2(a1 * c[4 + j] - b1 * sn[4 + j],
+                                        b1 * c[4 + j] + a1 * sn[4 + j]);
+            }
+          }
+          __nv_bfloat16* out = out_at(head);
+          *reinterpret_cast<uint4*>(out + e0) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+          *reinterpret_cast<uint4*>(out + e1) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+        }
+      }
     } else {
-      out[e0] = in[e0];
+      const bool turns = slot < half;
+      const int e0 = !turns ? half + slot : INTERLEAVED ? 2 * slot : slot;
+      const int e1 = INTERLEAVED ? e0 + 1 : e0 + half;
+      const float2 v = turns ? turn[t * half + slot] : make_float2(1.0f, 0.0f);
+      for (int head = group; head < a.heads; head += a.groups) {
+        const __nv_bfloat16* in = in_at(head);
+        __nv_bfloat16* out = out_at(head);
+        if (turns) {
+          const float x = __bfloat162float(in[e0]), y = __bfloat162float(in[e1]);
+          out[e0] = __float2bfloat16_rn(x * v.x - y * v.y);
+          out[e1] = __float2bfloat16_rn(y * v.x + x * v.y);
+        } else {
+          out[e0] = in[e0];
+        }
+      }
     }
   }
 }
@@ -156,8 +199,8 @@ __global__ void __launch_bounds__(256)
     rotary_tables_kernel(const RotaryArgs a, float* cos_out, float* sin_out) {
   b200::pdl_begin();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= a.work) return;
   const int half = a.rotary_dim / 2;
+  if (i >= a.tokens * half) return;
   const int pair = static_cast<int>(i % half);
   const int64_t token = i / half;
   float c, sn;
@@ -181,6 +224,7 @@ int plan_args(RotaryArgs& a, const void* positions, int64_t pos_stride_b, int64_
   a.pos64 = positions_64 != 0;
   a.turns = turns;
   a.gain = gain;
+  a.tokens = static_cast<int64_t>(batch) * seq;
   a.seq = seq;
   a.rotary_dim = rotary_dim;
   a.interleaved = interleaved != 0;
@@ -188,6 +232,7 @@ int plan_args(RotaryArgs& a, const void* positions, int64_t pos_stride_b, int64_
 }
 
 constexpr int64_t kMaxBlocks = 0x7fffffff;
+constexpr int kMaxRotary = 8192;  // 32 KB of angles a token
 
 }  // namespace
 
@@ -205,9 +250,9 @@ extern "C" int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h
                            batch, seq, rotary_dim, interleaved);
   if (st != B200_OK) return st;
   if (num_heads < 0 || num_kv_heads < 0 || head_dim < rotary_dim) return B200_ERR_INVALID_ARGUMENT;
-  const int64_t tokens = static_cast<int64_t>(batch) * seq;
   a.heads = num_heads + num_kv_heads;
-  if (tokens == 0 || a.heads == 0) return B200_OK;
+  if (a.tokens == 0 || a.heads == 0) return B200_OK;
+  if (rotary_dim > kMaxRotary) return B200_ERR_UNSUPPORTED;
   if ((num_heads > 0 && (!q || !q_out)) || (num_kv_heads > 0 && (!k || !k_out)))
     return B200_ERR_INVALID_ARGUMENT;
   a.heads_q = num_heads;
@@ -232,18 +277,27 @@ extern "C" int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h
     for (int64_t v : strides[i]) vec = vec && (v & 7) == 0;
   }
   a.slots = vec ? head_dim / 16 : rotary_dim / 2 + (head_dim - rotary_dim);
-  // threads that share a token's slot: 8 heads each, fewer when the tokens
-  // alone do not fill the GPU
-  a.groups = (a.heads + 7) / 8;
+  a.slot_threads = a.slots < 256 ? a.slots : 256;
+  // Tokens of a block: as many as still leave four blocks an SM, so that a
+  // decode step spreads over the GPU (64 tokens: one a block) and a prefill
+  // computes few angles twice (8 tokens a block, 10 heads a thread).
   const int sms = b200host::sm_count(b200host::current_device());
   if (sms <= 0) return B200_ERR_CUDA;
-  while (a.groups < a.heads && tokens * a.slots * a.groups < static_cast<int64_t>(sms) * 1024)
-    a.groups = a.groups * 2 < a.heads ? a.groups * 2 : a.heads;
-  a.work = tokens * a.slots * a.groups;
-  const int64_t blocks = (a.work + 255) / 256;
+  const int room = 256 / a.slot_threads;  // (token, head) places of a block
+  a.block_tokens = 1;
+  const int most = room / 8 >= a.heads ? 16 : 8;  // 16 where 8 leave a thread one head
+  while (a.block_tokens < most && a.block_tokens * 2 <= room &&
+         a.block_tokens * 2 * rotary_dim * 4 <= 32768 &&
+         a.tokens / (a.block_tokens * 2) >= static_cast<int64_t>(sms) * 4)
+    a.block_tokens *= 2;
+  a.groups = room / a.block_tokens < a.heads ? room / a.block_tokens : a.heads;
+  const int64_t blocks = (a.tokens + a.block_tokens - 1) / a.block_tokens;
   if (blocks > kMaxBlocks) return B200_ERR_INVALID_ARGUMENT;
-  const cudaError_t e = b200host::launch_pdl(vec ? rotary_vector_kernel : rotary_scalar_kernel,
-                                             dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
+  const int threads = (a.slot_threads * a.groups * a.block_tokens + 31) / 32 * 32;
+  const auto kernel = vec ? (interleaved ? rotary_kernel<true, true> : rotary_kernel<true, false>)
+                          : (interleaved ? rotary_kernel<false, true> : rotary_kernel<false, false>);
+  const cudaError_t e = b200host::launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads),
+                                             a.block_tokens * rotary_dim * 4,
                                              static_cast<cudaStream_t>(stream), a);
   return b200host::status_from_cuda(e);
 }
@@ -256,10 +310,10 @@ extern "C" int b200_rotary_tables(const void* positions, int64_t pos_stride_b,
   const int st = plan_args(a, positions, pos_stride_b, pos_stride_s, positions_64, turns, gain,
                            batch, seq, rotary_dim, interleaved);
   if (st != B200_OK) return st;
-  a.work = static_cast<int64_t>(batch) * seq * (rotary_dim / 2);
-  if (a.work == 0) return B200_OK;
+  const int64_t work = a.tokens * (rotary_dim / 2);
+  if (work == 0) return B200_OK;
   if (!cos_out || !sin_out) return B200_ERR_INVALID_ARGUMENT;
-  const int64_t blocks = (a.work + 255) / 256;
+  const int64_t blocks = (work + 255) / 256;
   if (blocks > kMaxBlocks) return B200_ERR_INVALID_ARGUMENT;
   const cudaError_t e = b200host::launch_pdl(rotary_tables_kernel,
                                              dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
