@@ -8,8 +8,14 @@ tokens each, decode replayed from CUDA graphs.  The reference serves this with
 its Scheduler, model.forward (prefill) and GraphRunner (decode)
 (bench_batched.py:150-200, qwen3/model.py:186-251, qwen3/graph_runner.py).
 
-The GEMMs, embedding, RMSNorms and the MLP are plain torch (cuBLAS): they are
-outside the attention hot path.  The attention path is this package's:
+By default the GEMMs, embedding, RMSNorms and the MLP are plain torch (cuBLAS):
+they are outside the attention hot path.  With ``layer_ops="bf16"`` or ``"fp8"``
+the whole decoder layer runs on the package's kernels: ``rms_norm`` (with the
+residual's addition before the MLP), ``linear`` (the gated activation and the
+second residual in its epilogue) and, in 8 bits, ``rms_norm_fp8`` and
+``quantize_rows_fp8`` in front of each product.  ``rope_plan`` scales the rotary
+frequencies for long contexts; ``qk_norm=False`` turns q and k by ``rotary``.
+The attention path is this package's in every case:
 
 * prefill (packed tokens of all requests): ``qk_norm_rope_kv_write`` (QK norm
   + RoPE), ``kv_scatter_slots`` (the prompt's K/V into the paged pool) and
@@ -36,6 +42,7 @@ import torch
 from . import ops
 from .graph_runner import GraphRunner
 from .paged_kv import KVCachePool, PagedKVCache
+from .rope import RotaryPlan
 
 QWEN3_0_6B = dict(layers=28, hidden=1024, heads=16, kv_heads=8, head_dim=128,
                   intermediate=3072, vocab=151936, rope_theta=1e6, eps=1e-6)
@@ -47,7 +54,8 @@ class Qwen3DecodeModel:
 
     def __init__(self, device, layers=28, hidden=1024, heads=16, kv_heads=8, head_dim=128,
                  intermediate=3072, vocab=151936, rope_theta=1e6, eps=1e-6, max_pos=4096,
-                 seed=0, std=0.02):
+                 seed=0, std=0.02, layer_ops="torch", rope_plan=None, qk_norm=True):
+        assert layer_ops in ("torch", "bf16", "fp8"), "layer_ops must be torch, bf16 or fp8"
         g = torch.Generator(device=device).manual_seed(seed)
         bf = torch.bfloat16
 
@@ -73,6 +81,53 @@ class Qwen3DecodeModel:
         emb = torch.cat([f, f], dim=-1)
         self.cos_t, self.sin_t = emb.cos(), emb.sin()                 # fp32 rows, as the reference
         self.scale = head_dim ** -0.5
+        self.layer_ops, self.qk_norm = layer_ops, qk_norm
+        self.plan = rope_plan if rope_plan is not None or qk_norm else \
+            RotaryPlan(head_dim, base=rope_theta, device=device)
+        if layer_ops != "torch":       # (out, in) rows, as ops.linear reads them
+            for ws in (self.wqkv, self.wo, self.wgu, self.wd):
+                for i, w_t in enumerate(ws):
+                    rows = w_t.t().contiguous()
+                    ws[i] = ops.quantize_rows_fp8(rows) if layer_ops == "fp8" else (rows, None)
+
+    def _normed(self, x, w, residual=None):
+        """RMS norm as a product's operand (rows, scale or None), and x + residual."""
+        if self.layer_ops == "fp8":
+            q, s, *h = ops.rms_norm_fp8(x, w, residual=residual, eps=self.eps)
+            return (q, s), h[0] if h else x
+        y = ops.rms_norm(x, w, residual=residual, eps=self.eps)
+        return ((y, None), x) if residual is None else ((y[0], None), y[1])
+
+    def _operand(self, x):
+        return ops.quantize_rows_fp8(x) if self.layer_ops == "fp8" else (x, None)
+
+    @staticmethod
+    def _product(x, w, **epilogue):
+        return ops.linear(x[0], w[0], x_scale=x[1], weight_scale=w[1], **epilogue)
+
+    def _block(self, i, h, attend):
+        """One decoder layer around ``attend(qkv) -> attention output``."""
+        if self.layer_ops == "torch":
+            h = h + attend(self._rms(h, self.ln1[i]) @ self.wqkv[i]) @ self.wo[i]
+            return self._mlp(i, h)
+        y, _ = self._normed(h, self.ln1[i])
+        o = attend(self._product(y, self.wqkv[i]))
+        o = self._product(self._operand(o), self.wo[i])
+        y, h = self._normed(o, self.ln2[i], residual=h)
+        a = self._product(y, self.wgu[i], gated=True, activation="silu")
+        return self._product(self._operand(a), self.wd[i], residual=h)
+
+    def _positions(self, positions):
+        """What ``_rotate`` needs of the step's (B, S) positions."""
+        if self.plan is None:
+            return self.cos_t[positions], self.sin_t[positions]
+        return ops.rotary_tables(positions, self.plan) if self.qk_norm else positions
+
+    def _rotate(self, i, q, k, v, at):
+        if not self.qk_norm:
+            return ops.rotary(q, k, at, self.plan)
+        return ops.qk_norm_rope_kv_write(q, k, v, self.qn[i], self.kn[i], at[0], at[1],
+                                         eps=self.eps, return_k=True)
 
     def _rms(self, x, w):
         xf = x.float()
@@ -84,6 +139,8 @@ class Qwen3DecodeModel:
         return h + (torch.nn.functional.silu(gate) * up) @ self.wd[i]
 
     def logits(self, h):
+        if self.layer_ops != "torch":
+            return ops.linear(ops.rms_norm(h, self.ln_f, eps=self.eps), self.embed)
         return self._rms(h, self.ln_f) @ self.embed.t()
 
     @torch.no_grad()
@@ -93,22 +150,21 @@ class Qwen3DecodeModel:
         returns the final hidden state of each sequence's last token."""
         H, Hkv, D = self.H, self.Hkv, self.D
         T = tokens.shape[0]
-        cos = self.cos_t[positions][None]          # (1, T, D)
-        sin = self.sin_t[positions][None]
+        at = self._positions(positions[None])
         h = self.embed[tokens][None]               # (1, T, hidden)
         for i in range(self.layers):
-            qkv = self._rms(h, self.ln1[i]) @ self.wqkv[i]
-            q = qkv[..., :H * D].view(1, T, H, D).transpose(1, 2)
-            k = qkv[..., H * D:(H + Hkv) * D].view(1, T, Hkv, D).transpose(1, 2)
-            v = qkv[..., (H + Hkv) * D:].view(1, T, Hkv, D).transpose(1, 2)
-            q, k = ops.qk_norm_rope_kv_write(q, k, v, self.qn[i], self.kn[i], cos, sin,
-                                             eps=self.eps, return_k=True)
-            k_t, v_t = k[0].transpose(0, 1), v[0].transpose(0, 1)   # (T, Hkv, D) views
-            ops.kv_scatter_slots(k_t, v_t, pool.k_buffer, pool.v_buffer, slots, i)
-            o = ops.flash_attention_prefill(q[0].transpose(0, 1), k_t, v_t, cu_seqlens,
-                                            self.scale, H, Hkv, D, max_seqlen=max_len)
-            h = h + o.reshape(1, T, H * D) @ self.wo[i]
-            h = self._mlp(i, h)
+            def attend(qkv):
+                q = qkv[..., :H * D].view(1, T, H, D).transpose(1, 2)
+                k = qkv[..., H * D:(H + Hkv) * D].view(1, T, Hkv, D).transpose(1, 2)
+                v = qkv[..., (H + Hkv) * D:].view(1, T, Hkv, D).transpose(1, 2)
+                q, k = self._rotate(i, q, k, v, at)
+                k_t, v_t = k[0].transpose(0, 1), v[0].transpose(0, 1)   # (T, Hkv, D) views
+                ops.kv_scatter_slots(k_t, v_t, pool.k_buffer, pool.v_buffer, slots, i)
+                o = ops.flash_attention_prefill(q[0].transpose(0, 1), k_t, v_t, cu_seqlens,
+                                                self.scale, H, Hkv, D, max_seqlen=max_len)
+                return o.reshape(1, T, H * D)
+
+            h = self._block(i, h, attend)
         return h[0, cu_seqlens[1:].long() - 1]     # (B, hidden)
 
     @torch.no_grad()
@@ -117,19 +173,18 @@ class Qwen3DecodeModel:
         positions, (B,) int32 rows -> (B, 1, vocab) logits.  Capture-safe."""
         B = input_ids.shape[0]
         H, Hkv, D = self.H, self.Hkv, self.D
-        cos = self.cos_t[position_ids]             # (B, 1, D)
-        sin = self.sin_t[position_ids]
+        at = self._positions(position_ids)
         h = self.embed[input_ids]                  # (B, 1, hidden)
         for i in range(self.layers):
-            qkv = self._rms(h, self.ln1[i]) @ self.wqkv[i]
-            q = qkv[..., :H * D].view(B, 1, H, D).transpose(1, 2)
-            k = qkv[..., H * D:(H + Hkv) * D].view(B, 1, Hkv, D).transpose(1, 2)
-            v = qkv[..., (H + Hkv) * D:].view(B, 1, Hkv, D).transpose(1, 2)
-            q, k = ops.qk_norm_rope_kv_write(q, k, v, self.qn[i], self.kn[i], cos, sin,
-                                             eps=self.eps, return_k=True)
-            o = ops.triton_paged_attention_decode_batch(q, k, v, caches, i, self.scale, row_ids)
-            h = h + o @ self.wo[i]
-            h = self._mlp(i, h)
+            def attend(qkv):
+                q = qkv[..., :H * D].view(B, 1, H, D).transpose(1, 2)
+                k = qkv[..., H * D:(H + Hkv) * D].view(B, 1, Hkv, D).transpose(1, 2)
+                v = qkv[..., (H + Hkv) * D:].view(B, 1, Hkv, D).transpose(1, 2)
+                q, k = self._rotate(i, q, k, v, at)
+                return ops.triton_paged_attention_decode_batch(q, k, v, caches, i, self.scale,
+                                                               row_ids)
+
+            h = self._block(i, h, attend)
         return self.logits(h)
 
 
