@@ -328,6 +328,10 @@ B200_DEVICE void st_global_v8(void* p, const uint32_t (&w)[8]) {
 B200_DEVICE float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 B200_DEVICE float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+B200_DEVICE void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<uint64_t>(p)));
+}
+
 // First statement of a kernel launched with b200host::launch_pdl: wait until
 // the previous kernel on the stream has completed and its writes are visible
 // (a no-op for an ordinary launch), then let the next programmatic dependent

@@ -31,6 +31,7 @@
 // roles give up too, outstanding copies are awaited and TMEM is freed.
 #include <mutex>
 
+#include "linear.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -49,24 +50,6 @@ constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at m
 constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s a pipeline wait
 constexpr uint64_t kDrainLimitNs = 100000000ull;   // 0.1 s a copy after a give-up
-
-struct LinearArgs {
-  const float* x_scale;  // nullable together
-  const float* w_scale;
-  const __nv_bfloat16* bias;      // nullable
-  const __nv_bfloat16* residual;  // nullable
-  __nv_bfloat16* out;
-  int64_t r_row, o_row;
-  int m, n;
-  int k_blocks;          // blocks of 128 bytes of K
-  int m_tiles, n_tiles;
-  int gated;             // 0, 1: boxes of 16 rows, 2: one 4-D box
-  int act;
-  int splits;            // CTAs of a cluster, each with a share of K
-  int stages;
-  int pairs;             // out and residual take 4-byte accesses
-  int32_t* dev_status;
-};
 
 struct __align__(8) Barriers {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -210,33 +193,6 @@ B200_DEVICE float ld_shared(uint32_t addr) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
-}
-
-// v / (1 + e^-v'): the quotient stays right at both ends (v' large and negative: 0)
-B200_DEVICE float gate_by(float v, float z) { return __fdividef(v, 1.0f + __expf(-z)); }
-
-template <int N>
-B200_DEVICE void activate(float (&v)[N], int act) {
-  switch (act) {  // outside the loops: one branch for N values
-    case B200_ACT_RELU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // NaN stays
-      break;
-    case B200_ACT_SILU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = gate_by(v[i], v[i]);
-      break;
-    case B200_ACT_GELU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
-      break;
-    case B200_ACT_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + e^-2z)
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = gate_by(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
-      break;
-    default: break;
-  }
 }
 
 struct Tile {
@@ -792,7 +748,7 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
                            const void* residual, int64_t r_stride, void* out, int64_t o_stride,
                            int m, int n, int k, int fp8, int gated, int activation,
                            int32_t* dev_status, void* stream) {
-  if (m < 0 || n <= 0 || k <= 0 || n > 0x3fffffff) return B200_ERR_INVALID_ARGUMENT;
+  if (m < 0 || n <= 0 || k <= 0 || n > 0x3fffffff || k > 0x1fffffff) return B200_ERR_INVALID_ARGUMENT;
   if (activation < B200_ACT_NONE || activation > B200_ACT_GELU_TANH)
     return B200_ERR_INVALID_ARGUMENT;
   if (m == 0) return B200_OK;
@@ -825,6 +781,10 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   const int dev = b200host::current_device();
   const int sms = b200host::sm_count(dev);
   if (sms <= 0) return B200_ERR_CUDA;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (b200host::linear_is_small(a, k, fp8 != 0))
+    return b200host::status_from_cuda(
+        b200host::linear_small(a, x, x_stride, w, w_stride, k, fp8 != 0, sms, cs));
   int st = ensure_smem_attr(dev);
   if (st != B200_OK) return st;
 
@@ -846,7 +806,6 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
                      gated ? 16 : kRows);
   if (st == B200_OK) st = encode_rows(&tx, x, m, k, x_stride, fp8 != 0, pair ? bn / 2 : bn);
   if (st != B200_OK) return st;
-  cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, pair, tw, tx, a, sms, cs)
                                         : launch_bn<false>(bn, pair, tw, tx, a, sms, cs));
 }

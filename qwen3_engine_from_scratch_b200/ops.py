@@ -858,6 +858,11 @@ def _stream_of(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _status_of(index: int) -> int:
+    t = _status.get(index)
+    return t.data_ptr() if t is not None else _status_ptr(torch.device("cuda", index))
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """(..., n) as (rows, n) with contiguous rows (a copy only where the strides need one)."""
     if t.dim() != 2:
@@ -888,8 +893,11 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
         if weight.stride(0) != 1:
             weight = weight.contiguous()
         w_ptr = weight.data_ptr()
-    x2 = _rows(x)
-    rows = x2.shape[0]
+    if x.is_contiguous():
+        x2, x_stride, rows = x, hidden, x.numel() // hidden
+    else:
+        x2 = _rows(x)
+        rows, x_stride = x2.shape[0], x2.stride(0)
     if out is None:
         y = x.new_empty(shape, dtype=FP8) if fp8 else \
             torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -906,8 +914,9 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
     if residual is not None:
         assert residual.shape == shape and residual.dtype == torch.bfloat16, \
             "residual must have x's shape, bf16"
-        r2 = _rows(residual)
-        r_ptr, r_stride = r2.data_ptr(), r2.stride(0)
+        r2 = residual if residual.is_contiguous() else _rows(residual)
+        r_ptr = r2.data_ptr()
+        r_stride = hidden if r2 is residual and r2.is_contiguous() else r2.stride(0)
         if residual_out is None:
             h, h_stride = torch.empty_like(x, memory_format=torch.contiguous_format), hidden
         else:
@@ -916,9 +925,9 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
         h_ptr = h.data_ptr()
     else:
         assert residual_out is None, "residual_out needs a residual"
-    st = _native.load().b200_rms_norm(x2.data_ptr(), x2.stride(0), r_ptr, r_stride, w_ptr,
+    st = _native.load().b200_rms_norm(x2.data_ptr(), x_stride, r_ptr, r_stride, w_ptr,
                                       y.data_ptr(), y_stride, s_ptr, h_ptr, h_stride, rows, hidden,
-                                      eps, _status_ptr(x.device), _stream_of(index))
+                                      eps, _status_of(index), _stream_of(index))
     if st:
         _native.check(st, what)
     if fp8:
@@ -1010,7 +1019,7 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
         assert weight_scale.dim() == 1 and weight_scale.shape[0] == wide and \
             weight_scale.dtype == torch.float32, \
             "weight_scale must be fp32, one for each row of weight"
-        x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+        x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()  # kept to the launch
         xs_ptr, ws_ptr = x_scale.data_ptr(), weight_scale.data_ptr()
     else:
         assert x_scale is None and weight_scale is None, "scales belong to fp8 operands"
@@ -1032,11 +1041,20 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
         y, y_stride = x.new_empty(shape, dtype=torch.bfloat16), n
     else:
         y, y_stride = out, max(n, _out_rows(out, shape, torch.bfloat16, index, "out").stride(0))
-    (x2, x_stride), (w2, w_stride) = _tma_rows(_rows(x)), _tma_rows(weight)
+    unit = 16 if fp8 else 8
+    if k % unit == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        x2, x_stride, m = x, k, x.numel() // k
+    else:
+        x2, x_stride = _tma_rows(_rows(x))
+        m = x2.shape[0]
+    if k % unit == 0 and weight.is_contiguous() and weight.data_ptr() % 16 == 0:
+        w2, w_stride = weight, k
+    else:
+        w2, w_stride = _tma_rows(weight)
     st = _native.load().b200_linear(
         x2.data_ptr(), x_stride, xs_ptr, w2.data_ptr(), w_stride, ws_ptr, b_ptr, r_ptr, r_stride,
-        y.data_ptr(), y_stride, x2.shape[0], n, k, fp8, gated, ACTIVATIONS[activation],
-        _status_ptr(x.device), _stream_of(index))
+        y.data_ptr(), y_stride, m, n, k, fp8, gated, ACTIVATIONS[activation], _status_of(index),
+        _stream_of(index))
     if st:
         _native.check(st, "b200_linear")
     return y

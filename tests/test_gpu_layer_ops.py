@@ -226,7 +226,9 @@ PRODUCT_SIZES = [(1, 8, 1), (1, 64, 128), (1, 1000, 257), (2, 16, 3), (5, 1024, 
                  (129, 320, 130), (200, 1001, 77), (257, 264, 1000), (300, 2048, 2050), (1, 12288, 16),
                  (17, 20000, 65), (511, 65, 511),
                  # enough tiles for pairs of CTAs: an odd number of weight tiles, ragged ends
-                 (257, 128, 9500), (600, 192, 6400), (1000, 72, 4999), (2049, 1024, 2048)]
+                 (257, 128, 9500), (600, 192, 6400), (1000, 72, 4999), (2049, 1024, 2048),
+                 # few tokens with a long K, and more weight than the direct kernel takes
+                 (8, 5001, 300), (7, 4104, 64), (13, 12288, 1024)]
 
 
 @pytest.mark.parametrize("m,k,n", PRODUCT_SIZES)
