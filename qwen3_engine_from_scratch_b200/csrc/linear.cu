@@ -149,6 +149,19 @@ B200_DEVICE void load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int
   }
 }
 
+B200_DEVICE void prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
+B200_DEVICE void prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
 template <bool PAIR>
 B200_DEVICE void tmem_alloc(uint32_t slot, uint32_t cols) {
   if constexpr (PAIR) {
@@ -186,13 +199,25 @@ B200_DEVICE uint32_t remote_smem(uint32_t addr, uint32_t rank) {
 B200_DEVICE void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-B200_DEVICE void st_remote(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+B200_DEVICE void st_remote(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
 }
-B200_DEVICE float ld_shared(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+B200_DEVICE float4 ld_shared(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
+}
+
+// Where 4 columns (quad) of a row lie in an exchange buffer [from rank][quad][row]
+// of 16 bytes: a warp's 32 rows are 512 bytes in one piece, there and back.
+// (Rows of own columns, 16 bytes every 4 own, took the network 2.4 times as long.)
+B200_DEVICE uint32_t exchange_at(int from, int row, int own, int quad) {
+  return static_cast<uint32_t>((from * (own >> 2) + quad) * kRows + row) * 16;
 }
 
 struct Tile {
@@ -342,6 +367,37 @@ struct Epilogue {
   }
 };
 
+// The columns of this CTA in a split product, N at a time: the partials of all
+// ranks in rank order, then the epilogue.
+template <int N>
+B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t exchange, int own,
+                              int token0, int warp, int lane, float* xs) {
+  const int row = (warp & 3) * 32 + lane;
+#pragma unroll 1
+  for (int c = (warp >> 2) * N; c < own && token0 + c < a.m; c += 2 * N) {
+    if (a.w_scale != nullptr) {
+      __syncwarp();
+      if (lane < N) xs[lane] = token0 + c + lane < a.m ? a.x_scale[token0 + c + lane] : 0.0f;
+      __syncwarp();
+    }
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+#pragma unroll 2
+    for (int from = 0; from < a.splits; ++from) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 p = ld_shared(exchange + exchange_at(from, row, own, (c + i) >> 2));
+        v[i] += p.x;
+        v[i + 1] += p.y;
+        v[i + 2] += p.z;
+        v[i + 3] += p.w;
+      }
+    }
+    ep.put_columns<N>(token0 + c, v, xs, [] {});
+  }
+}
+
 template <int BN, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
@@ -359,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t base = smem_u32(smem);
-  const uint32_t exchange = base + a.stages * kStageBytes;  // [from rank][column][row] fp32
+  const uint32_t exchange = base + a.stages * kStageBytes;
   auto full = [&](int s) { return smem_u32(&B.full[s]); };
   auto empty = [&](int s) { return smem_u32(&B.empty[s]); };
   auto acc_full = [&](int b) { return smem_u32(&B.acc_full[b]); };
@@ -388,28 +444,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = B.tmem_base;
-  pdl_begin();
-  // a pipeline already gave up: start no new work until the host clears the status
-  const bool aborted = a.dev_status != nullptr &&
-                       (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
-
   const int cluster = PAIR ? 2 : a.splits;
   const int rank = static_cast<int>(blockIdx.x) % cluster;
   const int first = static_cast<int>(blockIdx.x) / cluster;
   const int stride = static_cast<int>(gridDim.x) / cluster;
-  const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
   // PAIR: both CTAs work on all of K, for the first CTA's MMA lane
   const int kb0 =
       PAIR ? 0 : static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / a.splits);
   const int kb1 = PAIR ? a.k_blocks
                        : static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / a.splits);
 
+  const Tile first_tile = tile_at<BN, PAIR>(a, first, rank);
+  // a pipeline gave up before this launch: no new work until the host clears the
+  // status (read before the wait below: the load would be on every launch's path)
+  const bool aborted = a.dev_status != nullptr &&
+                       (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
+  const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
+  if (warp == kProducerWarp && lane == 0 && first < tiles && a.gated != 1) {
+    // The first weight tiles start towards L2 while the previous kernel drains (a
+    // prefetch returns no data: what that kernel still writes is read after the wait).
+    for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb) {
+      if (a.gated == 2) prefetch_4d(&tm_w, kb * kKElems, 0, 0, first_tile.n0 / 16);
+      else prefetch_2d(&tm_w, kb * kKElems, first_tile.n0);
+    }
+  }
+  pdl_begin();
+
   if (warp == kProducerWarp && lane == 0) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += stride) {
-      const Tile t = tile_at<BN, PAIR>(a, tile, rank);
+      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, rank);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = wait_or_flag(empty(stage), phase ^ 1, &B, a.dev_status))) break;
         // PAIR: both CTAs' copies count on the first CTA's barrier
@@ -487,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
-      const Tile t = tile_at<BN, PAIR>(a, tile, rank);
+      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, rank);
       const int buf = count & 1;
       const uint32_t acc = tmem + lane0 + buf * BN;
       const Epilogue ep(a, t.n0, warp, lane);
@@ -520,16 +586,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // column c belongs to rank c / own: into that CTA's exchange buffer
         const int own = BN / a.splits, shift = __ffs(own) - 1;
-        const uint32_t slot = exchange + (rank * own * kRows + (warp & 3) * 32 + lane) * 4;
+        const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
         for (int c = part * 32; c < BN; c += 64) {
           uint32_t r[32];
           tmem_ld32(acc + c, r);
           tmem_wait_ld(r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int to = (c + i) >> shift, col = (c + i) & (own - 1);
-            st_remote(remote_smem(slot + col * kRows * 4, to), r[i]);
+          for (int i = 0; i < 32; i += 4) {
+            const int to = (c + i) >> shift, quad = ((c + i) & (own - 1)) >> 2;
+            st_remote(remote_smem(exchange + exchange_at(rank, row, own, quad), to), r + i);
           }
         }
       }
@@ -540,25 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!PAIR && a.splits > 1) {  // one tile a cluster
     cluster_sync();
     if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
-      const Tile t = tile_at<BN, PAIR>(a, first, rank);
-      const Epilogue ep(a, t.n0, warp, lane);
       const int own = BN / a.splits;
-      const int token0 = t.token0 + rank * own;
-      for (int c = (warp >> 2) * 4; c < own; c += 8) {
-        if (token0 + c >= a.m) break;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int from = 0; from < a.splits; ++from) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] += ld_shared(exchange + ((from * own + c + i) * kRows + (warp & 3) * 32 + lane) * 4);
-        }
-        if (a.w_scale != nullptr) {
-          __syncwarp();
-          if (lane < 4) xs[warp][lane] = token0 + c + lane < a.m ? a.x_scale[token0 + c + lane] : 0.0f;
-          __syncwarp();
-        }
-        ep.put_columns<4>(token0 + c, v, xs[warp], [] {});
-      }
+      const int token0 = first_tile.token0 + rank * own;
+      const Epilogue ep(a, first_tile.n0, warp, lane);
+      // the two warps of a lane quarter take half of the columns each
+      if (own >= 64) finish_split<32>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      else if (own == 32) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      else if (own == 16) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      else finish_split<4>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
     }
   }
   tc_fence_before();
