@@ -12,9 +12,9 @@
 // columns, so the epilogue of one tile overlaps the product of the next.
 //   warps 0-7  epilogue: lane l of warp w owns accumulator lane 32 (w % 4) + l,
 //              of every other 32 token columns
-//   warp 8     TMA producer (one lane): 128-byte swizzled K-major tiles,
-//              128 weight rows and BN tokens x 128 bytes of K a stage
-//   warp 9     MMA issuer (one lane): 4 instructions a stage (K = 32 bytes)
+//   warps 8, 9 TMA producers of W and X: 128-byte swizzled K-major panels, 128
+//              weight rows and BN tokens x 128 bytes of K, one or two a stage
+//   warp 10    MMA issuer: 4 instructions a panel (K = 32 bytes each)
 // Gated: lanes 0-15 of every warp hold gate rows and lanes 16-31 the up rows
 // of the same 16 outputs, so the two meet by one shuffle; the tile's rows
 // come from one 4-D box (k, 16, gate/up, group) where n is a multiple of 16, or
@@ -39,17 +39,22 @@ namespace {
 using namespace b200;
 
 constexpr int kRows = 128;        // weight rows of a tile (TMEM lanes)
-constexpr int kKBytes = 128;      // bytes of K a stage: one swizzle row
-constexpr int kABytes = kRows * kKBytes;
-constexpr int kThreads = 320;
+constexpr int kKBytes = 128;      // bytes of K in a panel: one swizzle row
+constexpr int kAPanel = kRows * kKBytes;
+constexpr int kThreads = 352;
 constexpr int kEpilogueWarps = 8;
-constexpr int kProducerWarp = 8;
-constexpr int kMmaWarp = 9;
+constexpr int kWeightWarp = 8;
+constexpr int kTokenWarp = 9;
+constexpr int kMmaWarp = 10;
 constexpr int kMaxStages = 10;
 constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
 constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s a pipeline wait
 constexpr uint64_t kDrainLimitNs = 100000000ull;   // 0.1 s a copy after a give-up
+
+// Panels of a stage.  A stage costs its MMA warp about 400 clocks (the wait, the
+// issue, the commit), the MMAs of one panel 64 to 512: the narrow tiles take two.
+constexpr int panels(int bn) { return bn <= 128 ? 2 : 1; }
 
 struct __align__(8) Barriers {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -62,6 +67,22 @@ B200_DEVICE bool wait_or_flag(uint32_t bar, uint32_t parity, Barriers* B, int32_
   if (mbar_wait_abortable(bar, parity, dev_status, kWaitLimitNs)) return true;
   if (atomicExch(&B->error, 1) == 0) flag_error(dev_status, B200_DEV_TIMEOUT);
   return false;
+}
+
+// The same for a whole warp: true where every lane's wait ended in time.
+B200_DEVICE bool warp_wait(uint32_t bar, uint32_t parity, Barriers* B, int32_t* dev_status) {
+  return __all_sync(0xffffffffu, wait_or_flag(bar, parity, B, dev_status));
+}
+
+// One lane of a converged warp, the same on every call.
+B200_DEVICE bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r != 0;
 }
 
 // c format f32, a / b format bf16 (1) of kind::f16 or e4m3 (0) of kind::f8f6f4, both K-major
@@ -107,14 +128,14 @@ B200_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_
 }
 
 // every MMA issued so far by this thread is done: an arrival on `bar` (PAIR: on
-// the barrier at that place in both CTAs)
+// the barrier at that place in both CTAs of the pair, the first at rank `leader`)
 template <bool PAIR>
-B200_DEVICE void commit(uint32_t bar) {
+B200_DEVICE void commit(uint32_t bar, int leader) {
   if constexpr (PAIR) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
         "[%0], %1;" ::"r"(bar),
-        "h"(static_cast<uint16_t>(3))
+        "h"(static_cast<uint16_t>(3 << leader))
         : "memory");
   } else {
     umma_commit(bar);
@@ -227,10 +248,9 @@ struct Tile {
 // Tiles in groups of kGroupTokens token tiles: within a group the token tiles
 // of one weight tile come one after another, so the CTAs at work at a time
 // share few weight tiles and few token tiles in L2.
-// PAIR: a tile has twice the weight rows, and n0 is its second half in the
-// cluster's second CTA.
+// PAIR: a tile has twice the weight rows, and n0 is its half of this CTA.
 template <int BN, bool PAIR>
-B200_DEVICE Tile tile_at(const LinearArgs& a, int tile, int rank) {
+B200_DEVICE Tile tile_at(const LinearArgs& a, int tile, int half) {
   const int per_group = kGroupTokens * a.n_tiles;
   const int g = tile / per_group;
   const int first = g * kGroupTokens;
@@ -238,7 +258,7 @@ B200_DEVICE Tile tile_at(const LinearArgs& a, int tile, int rank) {
   const int rem = tile - g * per_group;
   Tile t;
   t.token0 = (first + rem % rows) * BN;
-  const int n_tile = PAIR ? rem / rows * 2 + rank : rem / rows;
+  const int n_tile = PAIR ? rem / rows * 2 + half : rem / rows;
   t.n0 = n_tile * (a.gated ? kRows / 2 : kRows);
   return t;
 }
@@ -406,9 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Barriers B;
   __shared__ __align__(16) float xs[kEpilogueWarps][128];  // token scales of a warp's columns
   constexpr int kBRows = PAIR ? BN / 2 : BN;  // tokens in this CTA's shared memory
-  constexpr int kBBytes = kBRows * kKBytes;
+  constexpr int kPanels = panels(BN);
+  constexpr int kBPanel = kBRows * kKBytes;
+  constexpr int kABytes = kPanels * kAPanel, kBBytes = kPanels * kBPanel;
   constexpr int kStageBytes = kABytes + kBBytes;
-  constexpr int kKElems = FP8 ? 128 : 64;
+  constexpr int kKElems = FP8 ? 128 : 64;  // of a panel
   constexpr uint32_t kTmemCols = 2 * BN;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), 2);
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -444,57 +466,71 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = B.tmem_base;
-  const int cluster = PAIR ? 2 : a.splits;
+  // a cluster: one tile, its K split among `splits` CTAs (PAIR: pairs of CTAs)
+  const int cluster = (PAIR ? 2 : 1) * a.splits;
   const int rank = static_cast<int>(blockIdx.x) % cluster;
+  const int half = PAIR ? rank & 1 : 0;
+  const int leader = PAIR ? rank & ~1 : 0;
+  const int part = PAIR ? rank >> 1 : rank;
   const int first = static_cast<int>(blockIdx.x) / cluster;
   const int stride = static_cast<int>(gridDim.x) / cluster;
-  // PAIR: both CTAs work on all of K, for the first CTA's MMA lane
-  const int kb0 =
-      PAIR ? 0 : static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / a.splits);
-  const int kb1 = PAIR ? a.k_blocks
-                       : static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / a.splits);
+  const int kb0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * part / a.splits);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (part + 1) / a.splits);
 
-  const Tile first_tile = tile_at<BN, PAIR>(a, first, rank);
+  const Tile first_tile = tile_at<BN, PAIR>(a, first, half);
   // a pipeline gave up before this launch: no new work until the host clears the
   // status (read before the wait below: the load would be on every launch's path)
   const bool aborted = a.dev_status != nullptr &&
                        (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
   const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
-  if (warp == kProducerWarp && lane == 0 && first < tiles && a.gated != 1) {
+  if (warp == kWeightWarp && lane == 0 && first < tiles && a.gated != 1) {
     // The first weight tiles start towards L2 while the previous kernel drains (a
     // prefetch returns no data: what that kernel still writes is read after the wait).
-    for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb) {
-      if (a.gated == 2) prefetch_4d(&tm_w, kb * kKElems, 0, 0, first_tile.n0 / 16);
-      else prefetch_2d(&tm_w, kb * kKElems, first_tile.n0);
+    for (int p = kb0 * kPanels; p < min(kb1, kb0 + a.stages) * kPanels; ++p) {
+      if (a.gated == 2) prefetch_4d(&tm_w, p * kKElems, 0, 0, first_tile.n0 / 16);
+      else prefetch_2d(&tm_w, p * kKElems, first_tile.n0);
     }
   }
   pdl_begin();
 
-  if (warp == kProducerWarp && lane == 0) {
+  // The producer and MMA warps run their loops whole and one elected lane issues:
+  // in a branch of a single lane every operand of a TMA or MMA instruction takes
+  // its own move to the uniform registers (550 clocks a stage, whatever its size).
+  if (warp == kWeightWarp || warp == kTokenWarp) {
+    const bool elected = elect_one();
+    const bool weights = warp == kWeightWarp;
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += stride) {
-      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, rank);
+      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, half);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = wait_or_flag(empty(stage), phase ^ 1, &B, a.dev_status))) break;
-        // PAIR: both CTAs' copies count on the first CTA's barrier
-        const uint32_t bar = PAIR ? remote_smem(full(stage), 0) : full(stage);
-        const uint32_t dst = base + stage * kStageBytes;
-        const int k0 = kb * kKElems;
-        if (!PAIR || rank == 0) mbar_arrive_expect_tx(full(stage), (PAIR ? 2 : 1) * kStageBytes);
-        if (a.gated == 2) {
-          load_4d<PAIR>(dst, &tm_w, bar, k0, 0, 0, t.n0 / 16);
-        } else if (a.gated == 1) {
+        if (!(ok = warp_wait(empty(stage), phase ^ 1, &B, a.dev_status))) break;
+        if (elected) {
+          // PAIR: both CTAs' copies count on the first CTA's barrier
+          const uint32_t bar = PAIR ? remote_smem(full(stage), leader) : full(stage);
+          const uint32_t dst = base + stage * kStageBytes;
+          if (half == 0)
+            mbar_arrive_expect_tx(full(stage), (PAIR ? 2 : 1) * (weights ? kABytes : kBBytes));
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            load_2d<PAIR>(dst + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
-            load_2d<PAIR>(dst + g * 4096 + 2048, &tm_w, bar, k0, a.n + t.n0 + g * 16);
+          for (int p = 0; p < kPanels; ++p) {  // (a panel past K's end arrives as zeros)
+            const int k0 = (kb * kPanels + p) * kKElems;
+            const uint32_t to = weights ? dst + p * kAPanel : dst + kABytes + p * kBPanel;
+            if (!weights) {
+              load_2d<PAIR>(to, &tm_x, bar, k0, t.token0 + half * kBRows);
+            } else if (a.gated == 2) {
+              load_4d<PAIR>(to, &tm_w, bar, k0, 0, 0, t.n0 / 16);
+            } else if (a.gated == 1) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                load_2d<PAIR>(to + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
+                load_2d<PAIR>(to + g * 4096 + 2048, &tm_w, bar, k0, a.n + t.n0 + g * 16);
+              }
+            } else {
+              load_2d<PAIR>(to, &tm_w, bar, k0, t.n0);
+            }
           }
-        } else {
-          load_2d<PAIR>(dst, &tm_w, bar, k0, t.n0);
         }
-        load_2d<PAIR>(dst + kABytes, &tm_x, bar, k0, t.token0 + (PAIR ? rank * kBRows : 0));
         ++issued;
         if (++stage == a.stages) {
           stage = 0;
@@ -505,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // After a give-up the copies in flight land before the shared memory goes
     // away (PAIR: the first CTA waits for both CTAs' copies, and the second stays
     // until the cluster barrier at the end).
-    if (!ok && (!PAIR || rank == 0)) {
+    if (!ok && half == 0) {
       for (int i = 0; i < min(issued, a.stages); ++i) {
         if (--stage < 0) {
           stage = a.stages - 1;
@@ -514,46 +550,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait_abortable(full(stage), phase, nullptr, kDrainLimitNs);
       }
     }
-  } else if (warp == kMmaWarp && lane == 0 && (!PAIR || rank == 0)) {
+  } else if (warp == kMmaWarp && half == 0) {
     constexpr uint32_t idesc = instruction<FP8>(PAIR ? 2 * kRows : kRows, BN);
+    const bool elected = elect_one();
+    const uint64_t desc0 = smem_desc(base, 16, 1024);  // + 16-byte units
     int stage = 0, count = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < tiles; tile += stride, ++count) {
       const int buf = count & 1;
-      if (!(ok = wait_or_flag(acc_empty(buf), ((count >> 1) & 1) ^ 1, &B, a.dev_status))) break;
+      if (!(ok = warp_wait(acc_empty(buf), ((count >> 1) & 1) ^ 1, &B, a.dev_status))) break;
       tc_fence_after();
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = wait_or_flag(full(stage), phase, &B, a.dev_status))) break;
+        if (!(ok = warp_wait(full(stage), phase, &B, a.dev_status))) break;
         tc_fence_after();
-        const uint32_t sa = base + stage * kStageBytes, sb = sa + kABytes;
+        if (elected) {
+          const uint64_t da = desc0 + static_cast<uint32_t>(stage * (kStageBytes / 16));
+          const uint64_t db = da + kABytes / 16;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma<FP8, PAIR>(tmem + buf * BN, smem_desc(sa + j * 32, 16, 1024),
-                         smem_desc(sb + j * 32, 16, 1024), idesc, kb > kb0 || j > 0 ? 1u : 0u);
-        commit<PAIR>(empty(stage));
+          for (int j = 0; j < 4 * kPanels; ++j)
+            mma<FP8, PAIR>(tmem + buf * BN, da + (j >> 2) * (kAPanel / 16) + 2 * (j & 3),
+                           db + (j >> 2) * (kBPanel / 16) + 2 * (j & 3), idesc,
+                           kb > kb0 || j > 0 ? 1u : 0u);
+          commit<PAIR>(empty(stage), leader);
+        }
         if (++stage == a.stages) {
           stage = 0;
           phase ^= 1;
         }
       }
-      if (ok) commit<PAIR>(acc_full(buf));
+      if (ok && elected) commit<PAIR>(acc_full(buf), leader);
     }
-  } else if (PAIR && warp == kMmaWarp && lane == 0) {
+  } else if (PAIR && warp == kMmaWarp && lane == 0 && a.splits == 1) {
     // Second CTA: passes on that its accumulators were read.  From here, not from
     // the epilogue: a release to the cluster waits for the thread's stores.
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
       const int buf = count & 1;
       if (!wait_or_flag(acc_empty(buf), (count >> 1) & 1, &B, a.dev_status)) break;
-      arrive_remote(remote_smem(acc_empty(buf), 0));
+      arrive_remote(remote_smem(acc_empty(buf), leader));
     }
   } else if (warp < kEpilogueWarps) {
-    const int part = warp >> 2;  // which of every two 32-column groups
+    const int side = warp >> 2;  // which of every two 32-column groups
     const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
-      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, rank);
+      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, half);
       const int buf = count & 1;
       const uint32_t acc = tmem + lane0 + buf * BN;
       const Epilogue ep(a, t.n0, warp, lane);
@@ -563,18 +605,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
-          const int c = part * 32 + j * 64 + lane;
+          const int c = side * 32 + j * 64 + lane;
           xs[warp][j * 32 + lane] = c < cols ? a.x_scale[t.token0 + c] : 0.0f;
         }
         __syncwarp();
       }
-      bool ok = wait_or_flag(acc_full(buf), (count >> 1) & 1, &B, a.dev_status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!warp_wait(acc_full(buf), (count >> 1) & 1, &B, a.dev_status)) break;
       tc_fence_after();
       if (a.splits == 1) {
 #pragma unroll 1
-        for (int c = part * 32, j = 0; c < cols; c += 64, j += 32) {
+        for (int c = side * 32, j = 0; c < cols; c += 64, j += 32) {
           float v[32];
           tmem_ld32(acc + c, reinterpret_cast<uint32_t*>(v));
           ep.put_columns<32>(t.token0 + c, v, &xs[warp][j],
@@ -584,18 +624,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty(buf));
       } else {
-        // column c belongs to rank c / own: into that CTA's exchange buffer
+        // column c belongs to part c / own: into that CTA's exchange buffer
         const int own = BN / a.splits, shift = __ffs(own) - 1;
         const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
-        for (int c = part * 32; c < BN; c += 64) {
+        for (int c = side * 32; c < BN; c += 64) {
           uint32_t r[32];
           tmem_ld32(acc + c, r);
           tmem_wait_ld(r);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const int to = (c + i) >> shift, quad = ((c + i) & (own - 1)) >> 2;
-            st_remote(remote_smem(exchange + exchange_at(rank, row, own, quad), to), r + i);
+            st_remote(remote_smem(exchange + exchange_at(part, row, own, quad),
+                                  PAIR ? 2 * to + half : to), r + i);
           }
         }
       }
@@ -603,11 +644,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   __syncwarp();
-  if (!PAIR && a.splits > 1) {  // one tile a cluster
+  if (a.splits > 1) {  // one tile a cluster
     cluster_sync();
     if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
       const int own = BN / a.splits;
-      const int token0 = first_tile.token0 + rank * own;
+      const int token0 = first_tile.token0 + part * own;
       const Epilogue ep(a, first_tile.n0, warp, lane);
       // the two warps of a lane quarter take half of the columns each
       if (own >= 64) finish_split<32>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
@@ -641,7 +682,7 @@ template <bool FP8>
 cudaError_t set_smem_attrs() {
   const cudaError_t es[] = {set_smem_attr<32, FP8, false>(), set_smem_attr<64, FP8, false>(),
                             set_smem_attr<128, FP8, false>(), set_smem_attr<256, FP8, false>(),
-                            set_smem_attr<256, FP8, true>()};
+                            set_smem_attr<128, FP8, true>(), set_smem_attr<256, FP8, true>()};
   for (cudaError_t e : es)
     if (e != cudaSuccess) return e;
   return cudaSuccess;
@@ -677,44 +718,44 @@ int ensure_smem_attr(int dev) {
   return B200_OK;
 }
 
-// How a product is cut: token tiles of bn, CTAs of a cluster that split K, or
-// pairs of CTAs with 256 x 256 tiles.
+// How a product is cut: token tiles of bn, 128 weight rows a CTA or 256 a pair of
+// CTAs, and K split among the CTAs or pairs of a cluster.
+struct Cut {
+  int bn;
+  bool pair;
+  int max_log;                        // K is split at most 2^max_log ways
+  float stage, epilogue, exchange;    // us
+};
+constexpr Cut kCuts[] = {
+    {32, false, 3, 0.26f, 0.5f, 0.8f},  {64, false, 3, 0.28f, 0.7f, 1.2f},
+    {128, false, 3, 0.31f, 1.2f, 2.5f}, {256, false, 0, 0.40f, 2.2f, 0.0f},
+    {128, true, 2, 0.24f, 1.2f, 2.5f},  {256, true, 0, 0.36f, 2.2f, 0.0f}};
+
 struct Plan {
   int bn, splits;
   bool pair;
 };
 
-// The cut with the least estimated time, from a model of measured launches
-// (us): 4 for a launch and its first loads; a stage of 128 bytes of K costs 0.26
-// to 0.40 with the tile's width (64 bytes a clock into an SM, then the MMAs);
-// the last tile's epilogue and, where K is split, the exchange are in the open.
-// It gives the measured best or comes within 10 % of it over 18 shapes from 1 to
-// 2048 tokens: 128 x 4096 x 4096 takes 14.5 us with K split 4 ways (bn 128)
-// and 22.6 without, 512 x 4096 x 4096 24.1 with bn 128 and 26.6 with 256,
-// 1024 x 4096 x 4096 27.7 in pairs and 43.9 with bn 128.
+// The cut with the least estimated time.
 Plan choose(int m, int n_tiles, int k_blocks, const int* resident) {
-  constexpr int kBn[] = {32, 64, 128, 256, 256};
-  constexpr float kStage[] = {0.26f, 0.28f, 0.31f, 0.40f, 0.36f};
-  constexpr float kEpilogue[] = {0.5f, 0.7f, 1.2f, 2.2f, 2.2f};
-  constexpr float kExchange[] = {0.8f, 1.2f, 3.7f};
   Plan best{32, 1, false};
   float least = 3.4e38f;
-  for (int i = 0; i < 5; ++i) {
-    const bool pair = i == 4;
-    const int64_t tiles = static_cast<int64_t>((m + kBn[i] - 1) / kBn[i]) *
-                          (pair ? (n_tiles + 1) / 2 : n_tiles);
-    for (int log = 0; log < (i < 3 ? 4 : 1); ++log) {
+  for (const Cut& c : kCuts) {
+    const int64_t tiles = static_cast<int64_t>((m + c.bn - 1) / c.bn) *
+                          (c.pair ? (n_tiles + 1) / 2 : n_tiles);
+    for (int log = 0; log <= c.max_log; ++log) {
       const int splits = 1 << log;
       if (splits > 1 && splits * 2 > k_blocks) break;
-      const int64_t room = pair ? resident[1] / 2 : resident[log] / splits;
-      if (room == 0) continue;
+      const int log_ctas = log + (c.pair ? 1 : 0);
+      const int64_t room = resident[log_ctas] >> log_ctas;
+      if (room == 0) break;
       const float waves = static_cast<float>((tiles + room - 1) / room);
       if (splits > 1 && waves > 1.0f) break;  // clusters that split K do not persist
-      const float t = 4.0f + waves * ((k_blocks + splits - 1) / splits) * kStage[i] + kEpilogue[i] +
-                      (splits > 1 ? kExchange[i] : 0.0f);
+      const float t = 4.0f + waves * ((k_blocks + splits - 1) / splits) * c.stage + c.epilogue +
+                      (splits > 1 ? c.exchange : 0.0f);
       if (t < least) {
         least = t;
-        best = Plan{kBn[i], splits, pair};
+        best = Plan{c.bn, splits, c.pair};
       }
     }
   }
@@ -758,11 +799,11 @@ int encode_gated(CUtensorMap* map, const void* base, int64_t n, int64_t k, int64
 template <int BN, bool FP8, bool PAIR>
 cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, int sms,
                    cudaStream_t stream) {
-  const int stage_bytes = kABytes + (PAIR ? BN / 2 : BN) * kKBytes;
+  const int stage_bytes = panels(BN) * (kAPanel + (PAIR ? BN / 2 : BN) * kKBytes);
   const int exchange = a.splits > 1 ? BN * kRows * 4 : 0;
   a.stages = (kSmemBudget - exchange) / stage_bytes;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int cluster = PAIR ? 2 : a.splits;
+  const int cluster = (PAIR ? 2 : 1) * a.splits;
   const int64_t ctas = static_cast<int64_t>(a.m_tiles) * a.n_tiles * cluster;
   // without a split of K the CTAs (or pairs) persist and take tiles in turn
   const int resident = PAIR ? g_resident[b200host::current_device()][1] : sms;
@@ -787,7 +828,9 @@ cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, i
 template <bool FP8>
 cudaError_t launch_bn(int bn, bool pair, const CUtensorMap& tw, const CUtensorMap& tx,
                       const LinearArgs& a, int sms, cudaStream_t stream) {
-  if (pair) return launch<256, FP8, true>(tw, tx, a, sms, stream);
+  if (pair)
+    return bn == 128 ? launch<128, FP8, true>(tw, tx, a, sms, stream)
+                     : launch<256, FP8, true>(tw, tx, a, sms, stream);
   switch (bn) {
     case 32: return launch<32, FP8, false>(tw, tx, a, sms, stream);
     case 64: return launch<64, FP8, false>(tw, tx, a, sms, stream);
@@ -826,7 +869,7 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   a.m = m;
   a.n = n;
   const int per = fp8 ? 128 : 64;
-  a.k_blocks = (k + per - 1) / per;
+  const int k_panels = (k + per - 1) / per;
   a.gated = !gated ? 0 : n % 16 == 0 ? 2 : 1;
   a.act = activation;
   a.dev_status = dev_status;
@@ -845,7 +888,8 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
 
   const int tile_n = gated ? kRows / 2 : kRows;
   a.n_tiles = (n + tile_n - 1) / tile_n;
-  const Plan plan = choose(m, a.n_tiles, a.k_blocks, g_resident[dev]);
+  const Plan plan = choose(m, a.n_tiles, k_panels, g_resident[dev]);
+  a.k_blocks = (k_panels + panels(plan.bn) - 1) / panels(plan.bn);
   const int bn = plan.bn;
   const bool pair = plan.pair;
   a.m_tiles = (m + bn - 1) / bn;

@@ -14,7 +14,7 @@ struct LinearArgs {
   __nv_bfloat16* out;
   int64_t r_row, o_row;
   int m, n;
-  int k_blocks;          // blocks of 128 bytes of K
+  int k_blocks;          // stages of K
   int m_tiles, n_tiles;
   int gated;             // 0, 1: boxes of 16 rows, 2: one 4-D box
   int act;
