@@ -722,7 +722,9 @@ int ensure_smem_attr(int dev) {
 // CTAs, and K split among the CTAs or pairs of a cluster.
 // The times (us) are fitted to 219 launches of 23 shapes (17 to 2048 tokens, K 300
 // to 12,288, both types): 4 for a launch, its first loads and its end; `panel` for
-// 128 bytes of K of a tile, or the weight's bytes at 5.6 TB/s where that is more;
+// 128 bytes of K of a tile, or the weight's bytes at 5.6 TB/s where that is more,
+// and a third of the other (256 rows of 151,936 logits: 81 us in pairs of 256, 95
+// in (128), whose main loops alone would both hide behind the weight);
 // `epilogue` for the last tile's, `exchange` where K is split.  Over the 23
 // shapes the choice is within 3 % of the best cut on average and 15 % at most:
 // 64 x 12288 x 4096 in e4m3 takes 13.0 us in (64, split 4), 16.7 in (64, split 2),
@@ -761,8 +763,8 @@ Plan choose(int m, int n_tiles, int k_panels, const int* resident) {
       const float waves = static_cast<float>((tiles + room - 1) / room);
       if (splits > 1 && waves > 1.0f) break;  // clusters that split K do not persist
       const float main = waves * ((k_panels + splits - 1) / splits) * c.panel;
-      const float t = 4.0f + (main > read ? main : read) + c.epilogue +
-                      (splits > 1 ? c.exchange : 0.0f);
+      const float t = 4.0f + (main > read ? main + 0.35f * read : read + 0.35f * main) +
+                      c.epilogue + (splits > 1 ? c.exchange : 0.0f);
       if (t < least) {
         least = t;
         best = Plan{c.bn, splits, c.pair};

@@ -842,20 +842,21 @@ FP8 = torch.float8_e4m3fn
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
-def _gpu_of(x: torch.Tensor, *others) -> int:
-    """The index of x's device: the current CUDA device (the kernels go to its
-    current stream), where every other given tensor lies too.  (Single calls of
-    these operators are bound by the host, so the checks use the cheap accessors.)"""
+# Single calls of these operators are bound by the host (a launch is about 3 of 11
+# us), so their checks use the cheap accessors.
+
+_BF16, _F32 = torch.bfloat16, torch.float32
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _gpu_of(x: torch.Tensor) -> int:
+    """The index of x's device, which must be the current one: the kernels go to
+    its current stream."""
     index = x.get_device()
     assert index >= 0, "b200 kernels need CUDA tensors"
-    assert index == torch.cuda.current_device(), "the tensors must be on the current CUDA device"
-    for t in others:
-        assert t is None or t.get_device() == index, f"every tensor must be on cuda:{index}"
+    assert index == _current_device(), "the tensors must be on the current CUDA device"
     return index
-
-
-def _stream_of(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _status_of(index: int) -> int:
@@ -882,15 +883,17 @@ def _out_rows(out, shape, dtype, index, name):
 
 def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
     shape = x.shape
-    assert x.dtype == torch.bfloat16 and len(shape) >= 1, "x must be (..., hidden) bf16"
+    assert x.dtype is _BF16 and len(shape) >= 1, "x must be (..., hidden) bf16"
     hidden = shape[-1]
     assert hidden > 0, "hidden must be positive"
-    index = _gpu_of(x, weight, residual)
-    w_ptr = None
+    index = _gpu_of(x)
+    w_ptr = s_ptr = r_ptr = h_ptr = scale = h = None
+    r_stride = h_stride = 0
     if weight is not None:
-        assert weight.dim() == 1 and weight.shape[0] == hidden and \
-            weight.dtype == torch.bfloat16, "weight must be (hidden,) bf16"
-        if weight.stride(0) != 1:
+        assert weight.dtype is _BF16 and weight.dim() == 1 and weight.shape[0] == hidden, \
+            "weight must be (hidden,) bf16"
+        assert weight.get_device() == index, f"weight must be on cuda:{index}"
+        if not weight.is_contiguous():
             weight = weight.contiguous()
         w_ptr = weight.data_ptr()
     if x.is_contiguous():
@@ -898,36 +901,37 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
     else:
         x2 = _rows(x)
         rows, x_stride = x2.shape[0], x2.stride(0)
-    if out is None:
-        y = x.new_empty(shape, dtype=FP8) if fp8 else \
-            torch.empty_like(x, memory_format=torch.contiguous_format)
-        y_stride = hidden
+    y_stride = hidden
+    if out is not None:
+        y, y_stride = out, _out_rows(out, shape, FP8 if fp8 else _BF16, index, "out").stride(0)
+    elif fp8:
+        y = x.new_empty(shape, dtype=FP8)
     else:
-        y, y_stride = out, _out_rows(out, shape, FP8 if fp8 else torch.bfloat16, index,
-                                     "out").stride(0)
-    scale = s_ptr = None
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if fp8:
-        scale = x.new_empty(shape[:-1], dtype=torch.float32)
+        scale = x.new_empty(shape[:-1], dtype=_F32)
         s_ptr = scale.data_ptr()
-    h = r2 = r_ptr = h_ptr = None
-    r_stride = h_stride = 0
     if residual is not None:
-        assert residual.shape == shape and residual.dtype == torch.bfloat16, \
+        assert residual.dtype is _BF16 and residual.shape == shape, \
             "residual must have x's shape, bf16"
-        r2 = residual if residual.is_contiguous() else _rows(residual)
-        r_ptr = r2.data_ptr()
-        r_stride = hidden if r2 is residual and r2.is_contiguous() else r2.stride(0)
-        if residual_out is None:
-            h, h_stride = torch.empty_like(x, memory_format=torch.contiguous_format), hidden
+        assert residual.get_device() == index, f"residual must be on cuda:{index}"
+        if residual.is_contiguous():
+            r2, r_stride = residual, hidden
         else:
-            h, h_stride = residual_out, _out_rows(residual_out, shape, torch.bfloat16, index,
+            r2 = _rows(residual)
+            r_stride = r2.stride(0)
+        r_ptr, h_stride = r2.data_ptr(), hidden
+        if residual_out is None:
+            h = torch.empty_like(x, memory_format=torch.contiguous_format)
+        else:
+            h, h_stride = residual_out, _out_rows(residual_out, shape, _BF16, index,
                                                   "residual_out").stride(0)
         h_ptr = h.data_ptr()
     else:
         assert residual_out is None, "residual_out needs a residual"
     st = _native.load().b200_rms_norm(x2.data_ptr(), x_stride, r_ptr, r_stride, w_ptr,
                                       y.data_ptr(), y_stride, s_ptr, h_ptr, h_stride, rows, hidden,
-                                      eps, _status_of(index), _stream_of(index))
+                                      eps, _status_of(index), _raw_stream(index))
     if st:
         _native.check(st, what)
     if fp8:
@@ -1000,8 +1004,8 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     """
     assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
     dtype = x.dtype
-    fp8 = dtype == FP8
-    assert (fp8 or dtype == torch.bfloat16) and weight.dtype == dtype, \
+    fp8 = dtype is FP8
+    assert (fp8 or dtype is _BF16) and weight.dtype is dtype, \
         "x and weight must both be bf16 or both float8_e4m3fn"
     lead = x.shape[:-1]
     assert weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1], \
@@ -1010,37 +1014,42 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     assert k > 0 and wide > 0 and (not gated or wide % 2 == 0), \
         "weight must not be empty (gated: gate rows and as many up rows)"
     n = wide // 2 if gated else wide
-    index = _gpu_of(x, weight, bias, residual, x_scale, weight_scale)
+    index = _gpu_of(x)
+    for t in (weight, bias, residual, x_scale, weight_scale):
+        assert t is None or t.get_device() == index, f"every tensor must be on cuda:{index}"
     xs_ptr = ws_ptr = b_ptr = r_ptr = None
     if fp8:
         assert x_scale is not None and weight_scale is not None, "fp8 operands need their scales"
-        assert x_scale.shape == lead and x_scale.dtype == torch.float32, \
+        assert x_scale.shape == lead and x_scale.dtype is _F32, \
             "x_scale must be fp32, one for each row of x"
         assert weight_scale.dim() == 1 and weight_scale.shape[0] == wide and \
-            weight_scale.dtype == torch.float32, \
+            weight_scale.dtype is _F32, \
             "weight_scale must be fp32, one for each row of weight"
         x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()  # kept to the launch
         xs_ptr, ws_ptr = x_scale.data_ptr(), weight_scale.data_ptr()
     else:
         assert x_scale is None and weight_scale is None, "scales belong to fp8 operands"
     if bias is not None:
-        assert bias.dim() == 1 and bias.shape[0] == wide and bias.dtype == torch.bfloat16, \
+        assert bias.dim() == 1 and bias.shape[0] == wide and bias.dtype is _BF16, \
             "bias must be bf16, one for each row of weight"
         bias = bias.contiguous()
         b_ptr = bias.data_ptr()
     shape = lead + (n,)
     r_stride = 0
     if residual is not None:
-        assert residual.shape == shape and residual.dtype == torch.bfloat16, \
+        assert residual.shape == shape and residual.dtype is _BF16, \
             "residual must have the result's shape, bf16"
-        r2 = _rows(residual)
-        if r2.shape[0] > 1 and r2.stride(0) < n:       # broadcast rows
-            r2 = r2.contiguous()
-        r_ptr, r_stride = r2.data_ptr(), max(n, r2.stride(0))
+        r2, r_stride = residual, n
+        if not residual.is_contiguous():
+            r2 = _rows(residual)
+            if r2.shape[0] > 1 and r2.stride(0) < n:       # broadcast rows
+                r2 = r2.contiguous()
+            r_stride = max(n, r2.stride(0))
+        r_ptr = r2.data_ptr()
     if out is None:
-        y, y_stride = x.new_empty(shape, dtype=torch.bfloat16), n
+        y, y_stride = x.new_empty(shape, dtype=_BF16), n
     else:
-        y, y_stride = out, max(n, _out_rows(out, shape, torch.bfloat16, index, "out").stride(0))
+        y, y_stride = out, max(n, _out_rows(out, shape, _BF16, index, "out").stride(0))
     unit = 16 if fp8 else 8
     if k % unit == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
         x2, x_stride, m = x, k, x.numel() // k
@@ -1054,34 +1063,28 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     st = _native.load().b200_linear(
         x2.data_ptr(), x_stride, xs_ptr, w2.data_ptr(), w_stride, ws_ptr, b_ptr, r_ptr, r_stride,
         y.data_ptr(), y_stride, m, n, k, fp8, gated, ACTIVATIONS[activation], _status_of(index),
-        _stream_of(index))
+        _raw_stream(index))
     if st:
         _native.check(st, "b200_linear")
     return y
 
 
-def _rotary_head(t, out, dims, name):
-    """Pointers, (b, h, s) strides and heads of q or k and its output."""
-    shape = t.shape
-    assert t.dtype == torch.bfloat16 and len(shape) == dims, \
-        f"{name} must be bf16, (T, heads, D) or (B, heads, S, D) like q"
+def _rotary_pair(t, out, dims, index, name):
+    """q or k and its output, checked: contiguous heads, the same sizes."""
+    assert t.dtype is _BF16 and t.dim() == dims and t.get_device() == index, \
+        f"{name} must be bf16, (T, heads, D) or (B, heads, S, D) like q, on cuda:{index}"
     if t.stride(-1) != 1:
         t = t.contiguous()
     if out is None:
-        out = torch.empty_like(t, memory_format=torch.contiguous_format)
-    else:
-        assert out.shape == shape and out.dtype == t.dtype and out.stride(-1) == 1, \
-            f"{name}_out must be like {name} with a contiguous head"
-    if dims == 3:
-        (s0, h0, _), (s1, h1, _) = t.stride(), out.stride()
-        b0 = b1 = 0
-    else:
-        (b0, h0, s0, _), (b1, h1, s1, _) = t.stride(), out.stride()
-    return t, out, (t.data_ptr(), b0, h0, s0), (out.data_ptr(), b1, h1, s1), shape[1]
+        return t, torch.empty_like(t, memory_format=torch.contiguous_format)
+    assert out.shape == t.shape and out.dtype is _BF16 and out.stride(-1) == 1 and \
+        out.get_device() == index, f"{name}_out must be like {name} with a contiguous head"
+    return t, out
 
 
 def _check_positions(positions, plan, index):
     assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
+    assert positions.get_device() == index, f"positions must be on cuda:{index}"
     assert plan.turns.get_device() == index, f"the plan must be on cuda:{index}"
 
 
@@ -1094,28 +1097,42 @@ def rotary(q, k, positions, plan, q_out=None, k_out=None):
     rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place).
     Any int32 or int64 position is exact to 2^-31 turns.
     """
-    dims, D = q.dim(), q.shape[-1]
+    dims = q.dim()
     assert dims in (3, 4), "q must be (T, heads, D) or (B, heads, S, D)"
-    assert plan.rotary_dim <= D, "the plan's rotary_dim exceeds head_dim"
-    index = _gpu_of(q, k, positions, q_out, k_out)
-    batch, seq = (1, q.shape[0]) if dims == 3 else (q.shape[0], q.shape[2])
-    q, q_out, q_in_args, q_out_args, heads = _rotary_head(q, q_out, dims, "q")
-    k_in_args = k_out_args = (None, 0, 0, 0)
-    kv_heads = 0
+    index = _gpu_of(q)
+    q, q_out = _rotary_pair(q, q_out, dims, index, "q")
     if k is not None:
-        k, k_out, k_in_args, k_out_args, kv_heads = _rotary_head(k, k_out, dims, "k")
-        assert k.shape[-1] == D and k.shape[0] == q.shape[0] and k.shape[-2 if dims == 4 else 0] == seq, \
-            "q and k must agree in all but their heads"
+        k, k_out = _rotary_pair(k, k_out, dims, index, "k")
     else:
         assert k_out is None, "k_out needs k"
     _check_positions(positions, plan, index)
-    assert tuple(positions.shape) == ((seq,) if dims == 3 else (batch, seq)), \
-        "positions must be (T,), or (B, S) for 4-D q"
+    kv_heads = kb = kh = ks = kob = koh = kos = 0
+    if dims == 3:
+        seq, heads, D = q.shape
+        batch, qb, qob, pb = 1, 0, 0, 0
+        (qs, qh, _), (qos, qoh, _) = q.stride(), q_out.stride()
+        if k is not None:
+            k_seq, kv_heads, k_dim = k.shape
+            (ks, kh, _), (kos, koh, _) = k.stride(), k_out.stride()
+            assert k_seq == seq and k_dim == D, "q and k must agree in all but their heads"
+        assert positions.dim() == 1 and positions.shape[0] == seq, "positions must be (T,)"
+    else:
+        batch, heads, seq, D = q.shape
+        (qb, qh, qs, _), (qob, qoh, qos, _) = q.stride(), q_out.stride()
+        if k is not None:
+            k_batch, kv_heads, k_seq, k_dim = k.shape
+            (kb, kh, ks, _), (kob, koh, kos, _) = k.stride(), k_out.stride()
+            assert k_batch == batch and k_seq == seq and k_dim == D, \
+                "q and k must agree in all but their heads"
+        assert positions.shape == (batch, seq), "positions must be (B, S)"
+        pb = positions.stride(0)
+    assert plan.rotary_dim <= D, "the plan's rotary_dim exceeds head_dim"
     st = _native.load().b200_rotary(
-        *q_in_args, *k_in_args, *q_out_args, *k_out_args, positions.data_ptr(),
-        positions.stride(0) if dims == 4 else 0, positions.stride(-1),
-        positions.dtype == torch.int64, plan.turns.data_ptr(), plan.gain, batch, seq, heads, kv_heads, D,
-        plan.rotary_dim, plan.interleaved, _stream_of(index))
+        q.data_ptr(), qb, qh, qs, k.data_ptr() if kv_heads else None, kb, kh, ks,
+        q_out.data_ptr(), qob, qoh, qos, k_out.data_ptr() if kv_heads else None, kob, koh, kos,
+        positions.data_ptr(), pb, positions.stride(-1), positions.dtype is torch.int64,
+        plan.turns.data_ptr(), plan.gain, batch, seq, heads, kv_heads, D, plan.rotary_dim,
+        plan.interleaved, _raw_stream(index))
     if st:
         _native.check(st, "b200_rotary")
     return q_out, k_out
@@ -1136,6 +1153,6 @@ def rotary_tables(positions, plan):
         positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
         positions.stride(-1), int(positions.dtype == torch.int64), plan.turns.data_ptr(),
         plan.gain, cos.data_ptr(), sin.data_ptr(), b, s, plan.rotary_dim, int(plan.interleaved),
-        _stream_of(index))
+        _raw_stream(index))
     _native.check(st, "b200_rotary_tables")
     return cos, sin
