@@ -1,16 +1,18 @@
 /*
  * qwen3_b200_attn.h -- C ABI of the B200 (sm_100a) attention hot path for the
- * Qwen3 inference engine (uphome/Qwen3-engine-from-scratch).
+ * Qwen3 inference engine (uphome/Qwen3-engine-from-scratch), and of the rest of
+ * its decoder layer: norms, matrix products, rotary positions.
  *
- * Three operations, each a hand-written CUDA kernel behind a plain-C entry
+ * Each operation is a hand-written CUDA kernel behind a plain-C entry
  * point: raw device pointers, element strides, sizes, a CUDA stream.  No torch
  * types cross this boundary.  All entry points only enqueue work on `stream`
  * (no host synchronisation, no allocation, grid sizes derived from shapes
- * only), so they can be captured in a CUDA graph.  The decode, prologue and
- * KV-scatter kernels are launched as programmatic dependents of the previous
- * kernel on `stream` (their CTAs may be scheduled while it drains); each one
- * waits for that kernel's completion before its first memory access, so the
- * stream order callers see is that of an ordinary launch.
+ * only), so they can be captured in a CUDA graph.  The decode, prologue,
+ * KV-scatter, norm, product and rotary kernels are launched as programmatic
+ * dependents of the previous kernel on `stream` (their CTAs may be scheduled
+ * while it drains); each one waits for that kernel's completion before it reads
+ * or writes a tensor (the products only prefetch weight lines to L2 before), so
+ * the stream order callers see is that of an ordinary launch.
  *
  * Conventions
  *   - bf16 tensors are passed as `const void*` / `void*` (2-byte elements).

@@ -363,7 +363,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Launch as a programmatic dependent of the previous kernel on the stream:
 // the grid may be scheduled while that kernel drains, which hides the launch
 // latency between back-to-back kernels.  The kernel must begin with
-// b200::pdl_begin() (nothing read or written before it).
+// b200::pdl_begin() (no tensor read or written before it).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                               cudaStream_t stream, Args&&... args) {

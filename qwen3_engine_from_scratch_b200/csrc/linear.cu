@@ -22,10 +22,22 @@
 // tokens before the store, so a lane writes two outputs (4 bytes) of one token
 // and a warp whole 32-byte sectors.
 //
-// Few tiles (a decode step): the CTAs of a cluster share one tile and split K;
-// every CTA sends its fp32 partial to the CTA that owns its token columns
+// Many tokens: pairs of CTAs (cta_group::2) compute 256 weight rows x 128 or 256
+// tokens, each with its own 128 weight rows and half of the tokens in shared
+// memory: 64 KB a panel where two single tiles of 256 tokens load 96.
+//
+// Few tiles (a decode step): the CTAs (or pairs) of a cluster share one tile and
+// split K; every CTA sends its fp32 partial to the CTA that owns its token columns
 // through distributed shared memory, and the owners add the partials in rank
-// order, so the result does not depend on timing.
+// order, so the result does not depend on timing.  Up to 16 tokens go to the
+// direct kernel of linear_small.cu.
+//
+// Bounds and what it measured (B200): large products by the tensor pipe, 95 %
+// active in bf16 and 91 % in e4m3 at the 1.5 GHz that the power cap leaves: 4096
+// tokens, 4096 -> 2 x 12288 gated with silu in 586 us (1.41 PFLOP/s) and 316 us
+// (2.61 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
+// of tiles: 81 us (4.8 TB/s).  64 x 12288 x 4096 in e4m3 by the weight's bytes and about 5 us
+// of launch, first loads, exchange and end: 12.4 us (4.2 TB/s).
 //
 // Every wait is bounded: one that runs out sets B200_DEV_TIMEOUT, the other
 // roles give up too, outstanding copies are awaited and TMEM is freed.

