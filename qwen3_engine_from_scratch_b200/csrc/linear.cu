@@ -10,17 +10,15 @@
 // 128-row tiles and pads only the small token side, and one kernel serves one
 // token and thousands.  Token tiles of BN columns; two accumulators of BN
 // columns, so the epilogue of one tile overlaps the product of the next.
-//   warps 0-7  epilogue: lane l of warp w owns accumulator lane 32 (w % 4) + l,
-//              of every other 32 token columns
-//   warps 8, 9 TMA producers of W and X: 128-byte swizzled K-major panels, 128
-//              weight rows and BN tokens x 128 bytes of K, one or two a stage
-//   warp 10    MMA issuer: 4 instructions a panel (K = 32 bytes each)
+//   warps 0-15   epilogue: lane l of warp w owns accumulator lane 32 (w % 4) + l,
+//                of every fourth 16 token columns
+//   warps 16, 17 TMA producers of W and X: 128-byte swizzled K-major panels, 128
+//                weight rows and BN tokens x 128 bytes of K, one or two a stage
+//   warp 18      MMA issuer: 4 instructions a panel (K = 32 bytes each)
 // Gated: lanes 0-15 of every warp hold gate rows and lanes 16-31 the up rows
 // of the same 16 outputs, so the two meet by one shuffle; the tile's rows
-// come from one 4-D box (k, 16, gate/up, group) where n is a multiple of 16, or
-// from 8 boxes of 16 rows.  Neighbouring lanes exchange values of neighbouring
-// tokens before the store, so a lane writes two outputs (4 bytes) of one token
-// and a warp whole 32-byte sectors.
+// come from one 4-D box (k, 16, gate/up, group), where n is no multiple of 16 the
+// last tile's from 8 boxes of 16 rows.
 //
 // Many tokens: pairs of CTAs (cta_group::2) compute 256 weight rows x 128 or 256
 // tokens, each with its own 128 weight rows and half of the tokens in shared
@@ -53,13 +51,16 @@ using namespace b200;
 constexpr int kRows = 128;        // weight rows of a tile (TMEM lanes)
 constexpr int kKBytes = 128;      // bytes of K in a panel: one swizzle row
 constexpr int kAPanel = kRows * kKBytes;
-constexpr int kThreads = 352;
-constexpr int kEpilogueWarps = 8;
-constexpr int kWeightWarp = 8;
-constexpr int kTokenWarp = 9;
-constexpr int kMmaWarp = 10;
+constexpr int kEpilogueWarps = 16;
+constexpr int kSides = kEpilogueWarps / 4;  // warps of a lane quarter
+constexpr int kCols = 16;                   // columns they take in turn
+constexpr int kThreads = (kEpilogueWarps + 3) * 32;
+constexpr int kScales = (256 + kSides * kCols - 1) / (kSides * kCols) * kCols;  // of a warp
+constexpr int kWeightWarp = kEpilogueWarps;
+constexpr int kTokenWarp = kWeightWarp + 1;
+constexpr int kMmaWarp = kTokenWarp + 1;
 constexpr int kMaxStages = 10;
-constexpr int kSmemBudget = 220 * 1024;  // dynamic shared memory of a CTA, at most
+constexpr int kSmemBudget = 204 * 1024;  // dynamic shared memory of a CTA, at most
 constexpr int kGroupTokens = 16;  // token tiles that take turns on the same weight rows
 constexpr uint64_t kWaitLimitNs = 1000000000ull;   // 1 s a pipeline wait
 constexpr uint64_t kDrainLimitNs = 100000000ull;   // 0.1 s a copy after a give-up
@@ -275,91 +276,197 @@ B200_DEVICE Tile tile_at(const LinearArgs& a, int tile, int half) {
   return t;
 }
 
+// Gated: whether the tile's 4 groups of 16 outputs are whole.
+B200_DEVICE bool whole_groups(const LinearArgs& a, int n0) { return n0 + kRows / 2 <= (a.n & ~15); }
+
+B200_DEVICE uint32_t even_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+B200_DEVICE uint32_t odd_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+
 // A lane's share of the epilogue of a tile: turns raw accumulators of this
-// lane's row into outputs.  Whole tiles take stores without bounds checks.
+// lane's row into outputs.  Rows of out that take 16-byte accesses go through a
+// buffer of the warp in shared memory ([two tokens][column] words of two bf16,
+// 16-byte units swizzled), so a lane stores 8 columns of one token; others take
+// 2-byte stores.  (By shuffles instead, at about 6 clocks of the SM each: 4.1
+// thousand clocks a 128 x 256 tile with 4-byte stores, 6.5 with 16-byte ones.)
 struct Epilogue {
   const LinearArgs& a;
+  uint32_t* buf;     // 256 words of this warp
   int lane, row_n;   // output column of this lane
-  int pair_n;        // first of the two output columns this lane writes
-  bool odd, high;    // odd lane of a pair / upper half-warp
-  bool whole;        // every column of the tile exists, 4-byte stores are aligned
+  int base_n;        // first output column of this warp
+  bool high;         // upper half-warp
   float w_scale, bias;
 
-  B200_DEVICE Epilogue(const LinearArgs& args, int n0, int warp, int l) : a(args), lane(l) {
-    const int quarter = warp & 3;
-    row_n = a.gated ? n0 + quarter * 16 + (l & 15) : n0 + quarter * 32 + l;
-    pair_n = row_n & ~1;
-    odd = l & 1;
+  B200_DEVICE Epilogue(const LinearArgs& args, int n0, int warp, int l, uint32_t* b)
+      : a(args), buf(b), lane(l) {
+    base_n = n0 + (warp & 3) * (a.gated ? 16 : 32);
+    row_n = base_n + (a.gated ? l & 15 : l);
     high = l >= 16;
-    whole = a.pairs && n0 + (a.gated ? kRows / 2 : kRows) <= a.n;
     const int w_row = a.gated && high ? a.n + row_n : row_n;
     const bool live = row_n < a.n;
     w_scale = a.w_scale != nullptr && live ? a.w_scale[w_row] : 1.0f;
     bias = a.bias != nullptr && live ? __bfloat162float(a.bias[w_row]) : 0.0f;
   }
 
-  // outputs (token, pair_n) and (token, pair_n + 1)
-  B200_DEVICE void put(int token, float lo, float hi) const {
-    if (token >= a.m || pair_n >= a.n) return;
-    __nv_bfloat16* o = a.out + token * a.o_row + pair_n;
-    const __nv_bfloat16* r =
-        a.residual != nullptr ? a.residual + token * a.r_row + pair_n : nullptr;
-    if (r != nullptr) lo += __bfloat162float(r[0]);
-    o[0] = __float2bfloat16_rn(lo);
-    if (pair_n + 1 < a.n) {
-      if (r != nullptr) hi += __bfloat162float(r[1]);
-      o[1] = __float2bfloat16_rn(hi);
+  // Any strides: v[i] is the output of column row_n and token + i * step.
+  template <int M>
+  B200_DEVICE void put_direct(int token, int step, float (&v)[M]) const {
+    const int tokens = row_n < a.n ? (a.m - token + step - 1) / step : 0;  // of this lane
+    if (a.residual != nullptr) {
+      const __nv_bfloat16* r = a.residual + token * a.r_row + row_n;
+#pragma unroll
+      for (int i = 0; i < M; ++i, r += step * a.r_row)
+        if (i < tokens) v[i] += __bfloat162float(*r);
     }
+    __nv_bfloat16* o = a.out + token * a.o_row + row_n;
+#pragma unroll
+    for (int i = 0; i < M; ++i, o += step * a.o_row)
+      if (i < tokens) *o = __float2bfloat16_rn(v[i]);
   }
 
-  // Values v[0..N) of this lane for the tokens token, token + step, ...: lanes
-  // 2i and 2i + 1 swap every other one, so that the even lane holds both
-  // outputs of the even tokens and the odd lane those of the odd ones.
-  template <int N>
-  B200_DEVICE void put_all(int token, int step, const float (&v)[N],
-                           const uint32_t (&res)[N / 2], bool fast) const {
-    const int first = token + (odd ? step : 0);
-    float lo[N / 2], hi[N / 2];
+  // 16-byte unit `unit` of the row of tokens 2 pair, 2 pair + 1 (plain: 32 words a row)
+  B200_DEVICE uint4* unit_at(int pair, int unit) const {
+    return reinterpret_cast<uint4*>(buf) + pair * 8 + (unit ^ (pair & 1));
+  }
+  B200_DEVICE uint32_t* word_at(int pair) const {
+    return reinterpret_cast<uint32_t*>(unit_at(pair, lane >> 2)) + (lane & 3);
+  }
+
+  // Plain: 16 tokens x 32 columns of the warp.  A lane loads and stores tokens
+  // 2 pair and 2 pair + 1 of 8 columns, pair = lane / 4.
+  struct Piece {
+    uint4 even, odd;
+  };
+  B200_DEVICE void fetch(int token, Piece& p) const {
+    const int t = token + (lane >> 2) * 2, n = base_n + (lane & 3) * 8;
+    p.even = p.odd = make_uint4(0, 0, 0, 0);
+    const __nv_bfloat16* r = a.residual + t * a.r_row + n;
+    if (n < a.n && t < a.m) p.even = *reinterpret_cast<const uint4*>(r);
+    if (n < a.n && t + 1 < a.m) p.odd = *reinterpret_cast<const uint4*>(r + a.r_row);
+  }
+  B200_DEVICE void put_plain(int token, float (&v)[16], const Piece& res) const {
+    const int pair = lane >> 2, unit = (lane & 3) * 2;
+    if (a.residual != nullptr) {
+      *unit_at(pair, unit) =
+          make_uint4(even_halves(res.even.x, res.odd.x), odd_halves(res.even.x, res.odd.x),
+                     even_halves(res.even.y, res.odd.y), odd_halves(res.even.y, res.odd.y));
+      *unit_at(pair, unit + 1) =
+          make_uint4(even_halves(res.even.z, res.odd.z), odd_halves(res.even.z, res.odd.z),
+                     even_halves(res.even.w, res.odd.w), odd_halves(res.even.w, res.odd.w));
+      __syncwarp();
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
-      lo[i] = odd ? got : v[2 * i];
-      hi[i] = odd ? v[2 * i + 1] : got;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = *word_at(i);
+        v[2 * i] += bf16_lo(w);
+        v[2 * i + 1] += bf16_hi(w);
+      }
     }
-    if (fast) {
-      if (a.residual != nullptr) {
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          lo[i] += bf16_lo(res[i]);
-          hi[i] += bf16_hi(res[i]);
+    for (int i = 0; i < 8; ++i) *word_at(i) = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    __syncwarp();
+    const uint4 x = *unit_at(pair, unit), y = *unit_at(pair, unit + 1);
+    __syncwarp();
+    const int t = token + pair * 2, n = base_n + (lane & 3) * 8;
+    __nv_bfloat16* o = a.out + t * a.o_row + n;
+    if (n < a.n && t < a.m)
+      *reinterpret_cast<uint4*>(o) = make_uint4(even_halves(x.x, x.y), even_halves(x.z, x.w),
+                                                even_halves(y.x, y.y), even_halves(y.z, y.w));
+    if (n < a.n && t + 1 < a.m)
+      *reinterpret_cast<uint4*>(o + a.o_row) =
+          make_uint4(odd_halves(x.x, x.y), odd_halves(x.z, x.w), odd_halves(y.x, y.y),
+                     odd_halves(y.z, y.w));
+  }
+
+  // Gated: 16 tokens x 16 columns.  v[j] is column row_n of token 2 j + high; rows
+  // of 16 words hold tokens 4 i + high and 4 i + 2 + high, and a lane loads and
+  // stores 4 columns of the two tokens of row lane / 4.
+  B200_DEVICE void fetch_gated(int token, Piece& p) const {
+    const int row = lane >> 2;
+    const int t = token + (row >> 1) * 4 + (row & 1), n = base_n + (lane & 3) * 4;
+    uint2 x = make_uint2(0, 0), y = make_uint2(0, 0);
+    const __nv_bfloat16* r = a.residual + t * a.r_row + n;
+    if (n < a.n && t < a.m) x = *reinterpret_cast<const uint2*>(r);
+    if (n < a.n && t + 2 < a.m) y = *reinterpret_cast<const uint2*>(r + 2 * a.r_row);
+    p.even = make_uint4(even_halves(x.x, y.x), odd_halves(x.x, y.x), even_halves(x.y, y.y),
+                        odd_halves(x.y, y.y));
+  }
+  B200_DEVICE void put_gated(int token, float (&v)[8], const Piece& res) const {
+    uint32_t* mine = buf + (high ? 16 : 0) + (lane & 15);  // + 32 a row pair
+    uint4* piece = reinterpret_cast<uint4*>(buf) + lane;
+    if (a.residual != nullptr) {
+      *piece = res.even;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] += bf16_lo(mine[32 * i]);
+        v[2 * i + 1] += bf16_hi(mine[32 * i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine[32 * i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    __syncwarp();
+    const uint4 x = *piece;
+    __syncwarp();
+    const int row = lane >> 2;
+    const int t = token + (row >> 1) * 4 + (row & 1), n = base_n + (lane & 3) * 4;
+    __nv_bfloat16* o = a.out + t * a.o_row + n;
+    if (n < a.n && t < a.m)
+      *reinterpret_cast<uint2*>(o) = make_uint2(even_halves(x.x, x.y), even_halves(x.z, x.w));
+    if (n < a.n && t + 2 < a.m)
+      *reinterpret_cast<uint2*>(o + 2 * a.o_row) =
+          make_uint2(odd_halves(x.x, x.y), odd_halves(x.z, x.w));
+  }
+
+  // Gated: the low half-warp holds gate rows and the high one up rows; each lane
+  // gives the other the values of half of the tokens and keeps a gate and an up
+  // value of tokens 2 j + high.
+  template <int N>
+  B200_DEVICE void meet(const float (&v)[N], float (&gate)[N / 2], float (&up)[N / 2]) const {
+    if constexpr (N == 16) {
+      // 32 bytes a lane through the buffer (units swizzled by 4 lanes)
+      const int to = lane * 2, from = (lane ^ 16) * 2, twist = (lane >> 2) & 1;
+      uint4* units = reinterpret_cast<uint4*>(buf);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = high ? v[2 * (4 * h + j)] : v[2 * (4 * h + j) + 1];
+        units[(to + h) ^ twist] = make_uint4(__float_as_uint(s[0]), __float_as_uint(s[1]),
+                                             __float_as_uint(s[2]), __float_as_uint(s[3]));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 u = units[(from + h) ^ twist];
+        const float got[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z),
+                              __uint_as_float(u.w)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = 4 * h + j;
+          gate[k] = high ? got[j] : v[2 * k];
+          up[k] = high ? v[2 * k + 1] : got[j];
         }
       }
-      __nv_bfloat16* o = a.out + first * a.o_row + pair_n;
-      const int64_t jump = 2 * step * a.o_row;
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i)
-        *reinterpret_cast<uint32_t*>(o + i * jump) = pack_bf16x2(lo[i], hi[i]);
+      __syncwarp();
     } else {
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) put(first + 2 * i * step, lo[i], hi[i]);
+      for (int i = 0; i < N / 2; ++i) {
+        const float got = __shfl_xor_sync(0xffffffffu, high ? v[2 * i] : v[2 * i + 1], 16);
+        gate[i] = high ? got : v[2 * i];
+        up[i] = high ? v[2 * i + 1] : got;
+      }
     }
   }
 
-  // accumulators of the tokens token .. token + N - 1; xs: their scales
+  // accumulators of the tokens token .. token + N - 1; xs: their scales; `wait`
+  // ends when they are there
   template <int N, class Wait>
   B200_DEVICE void put_columns(int token, float (&v)[N], const float* xs, Wait&& wait) const {
-    const bool fast = whole && token + N <= a.m;
-    constexpr int kMost = N / 2;
-    uint32_t res[kMost];
-    if (a.residual != nullptr && fast) {
-      // the residual's words of this lane, read while the accumulators come
-      const int step = a.gated ? 2 : 1;
-      const int first = token + (a.gated && high ? 1 : 0) + (odd ? step : 0);
-      const __nv_bfloat16* r = a.residual + first * a.r_row + pair_n;
-#pragma unroll
-      for (int i = 0; i < kMost; ++i)
-        if (!a.gated || i < kMost / 2)
-          res[i] = *reinterpret_cast<const uint32_t*>(r + 2 * i * step * a.r_row);
+    Piece res;
+    if constexpr (N == 16) {
+      if (a.wide && a.residual != nullptr) {  // read while the accumulators come
+        if (a.gated) fetch_gated(token, res);
+        else fetch(token, res);
+      }
     }
     wait();
     if (a.w_scale != nullptr) {
@@ -377,24 +484,27 @@ struct Epilogue {
       for (int i = 0; i < N; ++i) v[i] += bias;
     }
     if (a.gated) {
-      // low half-warp: gate, high half-warp: up; each keeps one token of two
       float gate[N / 2], up[N / 2];
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float got = __shfl_xor_sync(0xffffffffu, high ? v[2 * i] : v[2 * i + 1], 16);
-        gate[i] = high ? got : v[2 * i];
-        up[i] = high ? v[2 * i + 1] : got;
-      }
+      meet(v, gate, up);
       activate(gate, a.act);
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) gate[i] *= up[i];
-      uint32_t half[N / 4];
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) half[i] = res[i];
-      put_all<N / 2>(token + (high ? 1 : 0), 2, gate, half, fast);
+      if constexpr (N == 16) {
+        if (a.wide) {
+          put_gated(token, gate, res);
+          return;
+        }
+      }
+      put_direct(token + (high ? 1 : 0), 2, gate);
     } else {
       activate(v, a.act);
-      put_all<N>(token, 1, v, res, fast);
+      if constexpr (N == 16) {
+        if (a.wide) {
+          put_plain(token, v, res);
+          return;
+        }
+      }
+      put_direct(token, 1, v);
     }
   }
 };
@@ -406,7 +516,7 @@ B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t 
                               int token0, int warp, int lane, float* xs) {
   const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
-  for (int c = (warp >> 2) * N; c < own && token0 + c < a.m; c += 2 * N) {
+  for (int c = (warp >> 2) * N; c < own && token0 + c < a.m; c += kSides * N) {
     if (a.w_scale != nullptr) {
       __syncwarp();
       if (lane < N) xs[lane] = token0 + c + lane < a.m ? a.x_scale[token0 + c + lane] : 0.0f;
@@ -433,10 +543,11 @@ B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t 
 template <int BN, bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                  const LinearArgs a) {
+                  const __grid_constant__ CUtensorMap tm_g, const LinearArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Barriers B;
-  __shared__ __align__(16) float xs[kEpilogueWarps][128];  // token scales of a warp's columns
+  __shared__ __align__(16) uint32_t turn[kEpilogueWarps][256];  // outputs on their way
+  __shared__ __align__(16) float xs[kEpilogueWarps][kScales];  // token scales of a warp's columns
   constexpr int kBRows = PAIR ? BN / 2 : BN;  // tokens in this CTA's shared memory
   constexpr int kPanels = panels(BN);
   constexpr int kBPanel = kBRows * kKBytes;
@@ -469,6 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
+    if (a.gated) prefetch_tensormap(&tm_g);
   }
   if (warp == kMmaWarp) {
     tmem_alloc<PAIR>(smem_u32(&B.tmem_base), kTmemCols);
@@ -495,12 +607,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool aborted = a.dev_status != nullptr &&
                        (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
   const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
-  if (warp == kWeightWarp && lane == 0 && first < tiles && a.gated != 1) {
+  if (warp == kWeightWarp && lane == 0 && first < tiles) {
     // The first weight tiles start towards L2 while the previous kernel drains (a
     // prefetch returns no data: what that kernel still writes is read after the wait).
     for (int p = kb0 * kPanels; p < min(kb1, kb0 + a.stages) * kPanels; ++p) {
-      if (a.gated == 2) prefetch_4d(&tm_w, p * kKElems, 0, 0, first_tile.n0 / 16);
-      else prefetch_2d(&tm_w, p * kKElems, first_tile.n0);
+      if (!a.gated) prefetch_2d(&tm_w, p * kKElems, first_tile.n0);
+      else if (whole_groups(a, first_tile.n0))
+        prefetch_4d(&tm_g, p * kKElems, 0, 0, first_tile.n0 / 16);
     }
   }
   pdl_begin();
@@ -530,9 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t to = weights ? dst + p * kAPanel : dst + kABytes + p * kBPanel;
             if (!weights) {
               load_2d<PAIR>(to, &tm_x, bar, k0, t.token0 + half * kBRows);
-            } else if (a.gated == 2) {
-              load_4d<PAIR>(to, &tm_w, bar, k0, 0, 0, t.n0 / 16);
-            } else if (a.gated == 1) {
+            } else if (a.gated && whole_groups(a, t.n0)) {
+              load_4d<PAIR>(to, &tm_g, bar, k0, 0, 0, t.n0 / 16);
+            } else if (a.gated) {  // the last groups, or group, of 16
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 load_2d<PAIR>(to + g * 4096, &tm_w, bar, k0, t.n0 + g * 16);
@@ -603,22 +716,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       arrive_remote(remote_smem(acc_empty(buf), leader));
     }
   } else if (warp < kEpilogueWarps) {
-    const int side = warp >> 2;  // which of every two 32-column groups
+    const int side = warp >> 2;
     const uint32_t lane0 = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    constexpr int kTurn = kSides * kCols;
     int count = 0;
     for (int tile = first; tile < tiles; tile += stride, ++count) {
-      const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, half);
+      const Tile t = tile_at<BN, PAIR>(a, tile, half);
       const int buf = count & 1;
       const uint32_t acc = tmem + lane0 + buf * BN;
-      const Epilogue ep(a, t.n0, warp, lane);
-      constexpr int kGroups = (BN + 63) / 64;  // 32-column groups of this warp
+      const Epilogue ep(a, t.n0, warp, lane, turn[warp]);
+      constexpr int kGroups = (BN + kTurn - 1) / kTurn;  // groups of kCols columns of this warp
       const int cols = min(BN, a.m - t.token0);
       if (a.w_scale != nullptr && a.splits == 1) {
         __syncwarp();
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-          const int c = side * 32 + j * 64 + lane;
-          xs[warp][j * 32 + lane] = c < cols ? a.x_scale[t.token0 + c] : 0.0f;
+        for (int i = lane; i < kGroups * kCols; i += 32) {
+          const int c = side * kCols + i / kCols * kTurn + i % kCols;
+          xs[warp][i] = c < cols ? a.x_scale[t.token0 + c] : 0.0f;
         }
         __syncwarp();
       }
@@ -626,11 +739,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       if (a.splits == 1) {
 #pragma unroll 1
-        for (int c = side * 32, j = 0; c < cols; c += 64, j += 32) {
-          float v[32];
-          tmem_ld32(acc + c, reinterpret_cast<uint32_t*>(v));
-          ep.put_columns<32>(t.token0 + c, v, &xs[warp][j],
-                             [&] { tmem_wait_ld(reinterpret_cast<uint32_t*>(v)); });
+        for (int c = side * kCols, j = 0; c < cols; c += kTurn, j += kCols) {
+          float v[kCols];
+          tmem_ld16(acc + c, reinterpret_cast<uint32_t*>(v));
+          ep.put_columns<kCols>(t.token0 + c, v, &xs[warp][j],
+                                [&] { tmem_wait_ld16(reinterpret_cast<uint32_t*>(v)); });
         }
         tc_fence_before();
         __syncwarp();
@@ -640,12 +753,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int own = BN / a.splits, shift = __ffs(own) - 1;
         const int row = (warp & 3) * 32 + lane;
 #pragma unroll 1
-        for (int c = side * 32; c < BN; c += 64) {
-          uint32_t r[32];
-          tmem_ld32(acc + c, r);
-          tmem_wait_ld(r);
+        for (int c = side * kCols; c < BN; c += kTurn) {
+          uint32_t r[kCols];
+          tmem_ld16(acc + c, r);
+          tmem_wait_ld16(r);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
+          for (int i = 0; i < kCols; i += 4) {
             const int to = (c + i) >> shift, quad = ((c + i) & (own - 1)) >> 2;
             st_remote(remote_smem(exchange + exchange_at(part, row, own, quad),
                                   PAIR ? 2 * to + half : to), r + i);
@@ -661,10 +774,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
       const int own = BN / a.splits;
       const int token0 = first_tile.token0 + part * own;
-      const Epilogue ep(a, first_tile.n0, warp, lane);
-      // the two warps of a lane quarter take half of the columns each
-      if (own >= 64) finish_split<32>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
-      else if (own == 32) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      const Epilogue ep(a, first_tile.n0, warp, lane, turn[warp]);
+      // the warps of a lane quarter share the columns
+      if (own >= 32) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
       else if (own == 16) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
       else finish_split<4>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
     }
@@ -803,7 +915,7 @@ int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int
              : B200_ERR_TENSOR_MAP;
 }
 
-// gate and up rows as (k, 16, gate / up, group of 16): a box is a tile's 128 rows
+// gate and up rows as (k, 16, gate / up, whole group of 16): a box is a tile's 128 rows
 int encode_gated(CUtensorMap* map, const void* base, int64_t n, int64_t k, int64_t stride,
                  bool fp8) {
   const int size = fp8 ? 1 : 2;
@@ -821,7 +933,7 @@ int encode_gated(CUtensorMap* map, const void* base, int64_t n, int64_t k, int64
 }
 
 template <int BN, bool FP8, bool PAIR>
-cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, int sms,
+cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tg, LinearArgs a, int sms,
                    cudaStream_t stream) {
   const int stage_bytes = panels(BN) * (kAPanel + (PAIR ? BN / 2 : BN) * kKBytes);
   const int exchange = a.splits > 1 ? BN * kRows * 4 : 0;
@@ -846,20 +958,21 @@ cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, LinearArgs a, i
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, linear_kernel<BN, FP8, PAIR>, tw, tx, a);
+  return cudaLaunchKernelEx(&cfg, linear_kernel<BN, FP8, PAIR>, tw, tx, tg, a);
 }
 
 template <bool FP8>
 cudaError_t launch_bn(int bn, bool pair, const CUtensorMap& tw, const CUtensorMap& tx,
-                      const LinearArgs& a, int sms, cudaStream_t stream) {
+                      const CUtensorMap& tg, const LinearArgs& a, int sms,
+                      cudaStream_t stream) {
   if (pair)
-    return bn == 128 ? launch<128, FP8, true>(tw, tx, a, sms, stream)
-                     : launch<256, FP8, true>(tw, tx, a, sms, stream);
+    return bn == 128 ? launch<128, FP8, true>(tw, tx, tg, a, sms, stream)
+                     : launch<256, FP8, true>(tw, tx, tg, a, sms, stream);
   switch (bn) {
-    case 32: return launch<32, FP8, false>(tw, tx, a, sms, stream);
-    case 64: return launch<64, FP8, false>(tw, tx, a, sms, stream);
-    case 128: return launch<128, FP8, false>(tw, tx, a, sms, stream);
-    default: return launch<256, FP8, false>(tw, tx, a, sms, stream);
+    case 32: return launch<32, FP8, false>(tw, tx, tg, a, sms, stream);
+    case 64: return launch<64, FP8, false>(tw, tx, tg, a, sms, stream);
+    case 128: return launch<128, FP8, false>(tw, tx, tg, a, sms, stream);
+    default: return launch<256, FP8, false>(tw, tx, tg, a, sms, stream);
   }
 }
 
@@ -894,12 +1007,11 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   a.n = n;
   const int per = fp8 ? 128 : 64;
   const int k_panels = (k + per - 1) / per;
-  a.gated = !gated ? 0 : n % 16 == 0 ? 2 : 1;
+  a.gated = gated != 0;
   a.act = activation;
   a.dev_status = dev_status;
-  a.pairs = n % 2 == 0 && o_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0 &&
-            (residual == nullptr ||
-             (r_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(residual) & 3) == 0));
+  a.wide = n % 8 == 0 && o_stride % 8 == 0 && b200host::aligned16(out) &&
+           (residual == nullptr || (r_stride % 8 == 0 && b200host::aligned16(residual)));
   const int dev = b200host::current_device();
   const int sms = b200host::sm_count(dev);
   if (sms <= 0) return B200_ERR_CUDA;
@@ -921,14 +1033,15 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   if (pair) a.n_tiles = (a.n_tiles + 1) / 2;
   if (static_cast<int64_t>(a.m_tiles) * a.n_tiles > 0x0fffffff) return B200_ERR_INVALID_ARGUMENT;
 
-  CUtensorMap tw, tx;
-  if (a.gated == 2)
-    st = encode_gated(&tw, w, n, k, w_stride, fp8 != 0);
-  else
-    st = encode_rows(&tw, w, gated ? 2 * static_cast<int64_t>(n) : n, k, w_stride, fp8 != 0,
-                     gated ? 16 : kRows);
+  // gated: tw reads single groups of 16 rows, tg whole tiles of gate and up rows
+  CUtensorMap tw, tx, tg;
+  st = encode_rows(&tw, w, gated ? 2 * static_cast<int64_t>(n) : n, k, w_stride, fp8 != 0,
+                   gated ? 16 : kRows);
+  const bool whole_tiles = gated && n >= kRows / 2;
+  if (st == B200_OK && whole_tiles) st = encode_gated(&tg, w, n, k, w_stride, fp8 != 0);
+  if (!whole_tiles) tg = tw;
   if (st == B200_OK) st = encode_rows(&tx, x, m, k, x_stride, fp8 != 0, pair ? bn / 2 : bn);
   if (st != B200_OK) return st;
-  return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, pair, tw, tx, a, sms, cs)
-                                        : launch_bn<false>(bn, pair, tw, tx, a, sms, cs));
+  return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, pair, tw, tx, tg, a, sms, cs)
+                                        : launch_bn<false>(bn, pair, tw, tx, tg, a, sms, cs));
 }

@@ -16,11 +16,11 @@ struct LinearArgs {
   int m, n;
   int k_blocks;          // stages of K
   int m_tiles, n_tiles;
-  int gated;             // 0, 1: boxes of 16 rows, 2: one 4-D box
+  int gated;
   int act;
   int splits;            // CTAs of a cluster, each with a share of K
   int stages;
-  int pairs;             // out and residual take 4-byte accesses
+  int wide;              // out and residual take 16-byte accesses
   int32_t* dev_status;
 };
 
