@@ -422,12 +422,25 @@ int b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t
  * residual (m, n), out (m, n) bf16; x_scale, w_scale, bias and residual are
  * NULL where unused.  Row strides in elements, rows contiguous; x and w start on
  * 16 bytes and their row strides are multiples of 16 bytes (k itself need not
- * be); out may be residual.  Sums in fp32, one rounding.
+ * be); out may be residual, and overlaps nothing else.  Sums in fp32, one
+ * rounding.
  */
 int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
                 int64_t w_stride, const float* w_scale, const void* bias, const void* residual,
                 int64_t r_stride, void* out, int64_t o_stride, int m, int n, int k, int fp8,
                 int gated, int activation, int32_t* dev_status, void* stream);
+
+/* b200_linear of at most 8 tokens whose x and w may lie at any address and stride. */
+int b200_linear_unaligned(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+                          int64_t w_stride, const float* w_scale, const void* bias,
+                          const void* residual, int64_t r_stride, void* out, int64_t o_stride,
+                          int m, int n, int k, int fp8, int gated, int activation,
+                          int32_t* dev_status, void* stream);
+
+/* Rows of row_bytes bytes at any address and stride (in bytes) to rows on 16-byte
+ * boundaries, zero up to the next multiple of 16 bytes: operands for b200_linear. */
+int b200_pack_rows(const void* src, int64_t src_stride, void* dst, int64_t dst_stride,
+                   int64_t rows, int row_bytes, void* stream);
 
 /*
  * Rotary positions of q (batch, num_heads, seq, head_dim) and k (batch,

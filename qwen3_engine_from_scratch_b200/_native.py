@@ -93,6 +93,9 @@ SIGNATURES = {
     "b200_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I, _F, _P, _P]),
     "b200_linear": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64,
                          _I, _I, _I, _I, _I, _I, _P, _P]),
+    "b200_linear_unaligned": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64,
+                                   _I, _I, _I, _I, _I, _I, _P, _P]),
+    "b200_pack_rows": (_I, [_P, _I64, _P, _I64, _I64, _I, _P]),
     "b200_rotary": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                          _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                          _P, _I64, _I64, _I, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P]),

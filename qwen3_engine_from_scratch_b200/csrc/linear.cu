@@ -978,11 +978,56 @@ cudaError_t launch_bn(int bn, bool pair, const CUtensorMap& tw, const CUtensorMa
 
 }  // namespace
 
-extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
-                           int64_t w_stride, const float* w_scale, const void* bias,
-                           const void* residual, int64_t r_stride, void* out, int64_t o_stride,
-                           int m, int n, int k, int fp8, int gated, int activation,
-                           int32_t* dev_status, void* stream) {
+namespace {
+
+// dst rows (16-byte aligned, zero to the next multiple of 16 bytes) from src rows
+// at any address; a thread moves 16 bytes
+__global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* src, int64_t src_stride,
+                                                        uint8_t* dst, int64_t dst_stride, int64_t rows,
+                                                        int row_bytes, int pieces) {
+  pdl_begin();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t row = i / pieces;
+  if (row >= rows) return;
+  const int at = static_cast<int>(i - row * pieces) * 16;
+  const uint8_t* from = src + row * src_stride + at;
+  uint4 v;
+  if (at + 16 <= row_bytes) {
+    v = load_unaligned16(from);
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 15; ++b)
+      if (at + b < row_bytes) w[b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  *reinterpret_cast<uint4*>(dst + row * dst_stride + at) = v;
+}
+
+}  // namespace
+
+extern "C" int b200_pack_rows(const void* src, int64_t src_stride, void* dst, int64_t dst_stride,
+                              int64_t rows, int row_bytes, void* stream) {
+  if (rows < 0 || row_bytes <= 0 || row_bytes > 0x7fffffe0) return B200_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return B200_OK;
+  const int pieces = (row_bytes + 15) / 16;
+  if (!src || !dst || dst_stride < static_cast<int64_t>(pieces) * 16) return B200_ERR_INVALID_ARGUMENT;
+  if (!b200host::aligned16(dst) || dst_stride % 16) return B200_ERR_ALIGNMENT;
+  const int64_t blocks = (rows * pieces + 255) / 256;
+  if (blocks > 0x7fffffff) return B200_ERR_INVALID_ARGUMENT;
+  return b200host::status_from_cuda(b200host::launch_pdl(
+      pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
+      static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(src), src_stride,
+      static_cast<uint8_t*>(dst), dst_stride, rows, row_bytes, pieces));
+}
+
+namespace {
+
+int linear_any(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+               int64_t w_stride, const float* w_scale, const void* bias,
+               const void* residual, int64_t r_stride, void* out, int64_t o_stride,
+               int m, int n, int k, int fp8, int gated, int activation,
+               int32_t* dev_status, void* stream, bool any_address) {
   if (m < 0 || n <= 0 || k <= 0 || n > 0x3fffffff || k > 0x1fffffff) return B200_ERR_INVALID_ARGUMENT;
   if (activation < B200_ACT_NONE || activation > B200_ACT_GELU_TANH)
     return B200_ERR_INVALID_ARGUMENT;
@@ -990,8 +1035,9 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   if (!x || !w || !out) return B200_ERR_INVALID_ARGUMENT;
   if (fp8 ? !x_scale || !w_scale : x_scale || w_scale) return B200_ERR_INVALID_ARGUMENT;
   const int64_t unit = fp8 ? 16 : 8;  // elements of 16 bytes
-  if (!b200host::aligned16(x) || !b200host::aligned16(w) || x_stride % unit || w_stride % unit)
-    return B200_ERR_ALIGNMENT;
+  if (!any_address &&
+      (!b200host::aligned16(x) || !b200host::aligned16(w) || x_stride % unit || w_stride % unit))
+    return B200_ERR_ALIGNMENT;  // the tensor maps' rule; b200_pack_rows lays rows out
   if (x_stride < k || w_stride < k || o_stride < n || (residual && r_stride < n))
     return B200_ERR_INVALID_ARGUMENT;
 
@@ -1044,4 +1090,25 @@ extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale
   if (st != B200_OK) return st;
   return b200host::status_from_cuda(fp8 ? launch_bn<true>(bn, pair, tw, tx, tg, a, sms, cs)
                                         : launch_bn<false>(bn, pair, tw, tx, tg, a, sms, cs));
+}
+
+}  // namespace
+
+extern "C" int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+                           int64_t w_stride, const float* w_scale, const void* bias,
+                           const void* residual, int64_t r_stride, void* out, int64_t o_stride,
+                           int m, int n, int k, int fp8, int gated, int activation,
+                           int32_t* dev_status, void* stream) {
+  return linear_any(x, x_stride, x_scale, w, w_stride, w_scale, bias, residual, r_stride, out,
+                    o_stride, m, n, k, fp8, gated, activation, dev_status, stream, false);
+}
+
+extern "C" int b200_linear_unaligned(const void* x, int64_t x_stride, const float* x_scale, const void* w,
+                                     int64_t w_stride, const float* w_scale, const void* bias,
+                                     const void* residual, int64_t r_stride, void* out, int64_t o_stride,
+                                     int m, int n, int k, int fp8, int gated, int activation,
+                                     int32_t* dev_status, void* stream) {
+  if (m > 8) return B200_ERR_UNSUPPORTED;
+  return linear_any(x, x_stride, x_scale, w, w_stride, w_scale, bias, residual, r_stride, out,
+                    o_stride, m, n, k, fp8, gated, activation, dev_status, stream, true);
 }

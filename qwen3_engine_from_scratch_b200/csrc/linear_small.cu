@@ -45,9 +45,10 @@ B200_DEVICE void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 }
 
 // 16 bytes of a row from byte `at` on, zero past its end
-template <bool FP8>
+template <bool FP8, bool ALIGNED>
 B200_DEVICE uint4 piece(const uint8_t* row, int at, int end) {
-  if (at + 16 <= end) return *reinterpret_cast<const uint4*>(row + at);
+  if (at + 16 <= end)
+    return ALIGNED ? *reinterpret_cast<const uint4*>(row + at) : load_unaligned16(row + at);
   uint4 w = make_uint4(0, 0, 0, 0);
   if (at < end) {
     uint64_t lo = 0, hi = 0;
@@ -65,7 +66,7 @@ B200_DEVICE uint4 piece(const uint8_t* row, int at, int end) {
 }
 
 // TT token tiles of 8; a warp reads AHEAD steps before it multiplies the first
-template <int TT, int AHEAD, bool FP8>
+template <int TT, int AHEAD, bool FP8, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs a) {
   __shared__ float sums[kWarps][kRows][TT * 8 + 1];
   const LinearArgs& e = a.e;
@@ -99,10 +100,10 @@ __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs 
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) {
       const int at = k0 + s * kWarps * kStep + t * 16;
-      wv[s][0] = piece<FP8>(w[0], at, a.k_bytes);
-      wv[s][1] = piece<FP8>(w[1], at, a.k_bytes);
+      wv[s][0] = piece<FP8, ALIGNED>(w[0], at, a.k_bytes);
+      wv[s][1] = piece<FP8, ALIGNED>(w[1], at, a.k_bytes);
 #pragma unroll
-      for (int i = 0; i < TT; ++i) xv[s][i] = piece<FP8>(x[i], at, a.k_bytes);
+      for (int i = 0; i < TT; ++i) xv[s][i] = piece<FP8, ALIGNED>(x[i], at, a.k_bytes);
     }
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s)
@@ -142,11 +143,11 @@ __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs 
   }
 }
 
-template <int TT, int AHEAD>
+template <int TT, int AHEAD, bool ALIGNED>
 cudaError_t launch(const SmallArgs& a, bool fp8, unsigned blocks, cudaStream_t stream) {
-  return b200host::launch_pdl(
-      fp8 ? linear_small_kernel<TT, AHEAD, true> : linear_small_kernel<TT, AHEAD, false>,
-      dim3(blocks), dim3(kThreads), 0, stream, a);
+  return b200host::launch_pdl(fp8 ? linear_small_kernel<TT, AHEAD, true, ALIGNED>
+                                  : linear_small_kernel<TT, AHEAD, false, ALIGNED>,
+                              dim3(blocks), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -174,13 +175,17 @@ cudaError_t linear_small(const b200::LinearArgs& e, const void* x, int64_t x_str
   a.k_bytes = k * size;
   const int tile_n = e.gated ? kRows / 2 : kRows;
   const unsigned blocks = static_cast<unsigned>((e.n + tile_n - 1) / tile_n);
-  if (e.m > 8) return launch<2, 4>(a, fp8, blocks, stream);
+  const bool aligned = aligned16(x) && aligned16(w) && a.x_row % 16 == 0 && a.w_row % 16 == 0;
+  if (!aligned)
+    return e.m > 8 ? launch<2, 4, false>(a, fp8, blocks, stream)
+                   : launch<1, 4, false>(a, fp8, blocks, stream);
+  if (e.m > 8) return launch<2, 4, true>(a, fp8, blocks, stream);
   // Eight steps ahead where few blocks have to keep the memory busy and K feeds
   // them: 8 x 4096 x 1024 6.3 -> 5.4 us, 8 x 12288 x 4096 23.3 -> 20.7; with more
   // blocks than two an SM the registers cost more (8 x 4096 x 6144 10.7 -> 14.4).
   if (blocks <= 2u * sms && a.k_bytes >= 8 * kWarps * kStep)
-    return launch<1, 8>(a, fp8, blocks, stream);
-  return launch<1, 4>(a, fp8, blocks, stream);
+    return launch<1, 8, true>(a, fp8, blocks, stream);
+  return launch<1, 4, true>(a, fp8, blocks, stream);
 }
 
 }  // namespace b200host

@@ -968,21 +968,24 @@ def quantize_rows_fp8(x, out=None):
     return _norm(x, None, None, 0.0, True, out, None, "b200_rms_norm")
 
 
-def _tma_rows(t: torch.Tensor):
-    """2-D ``t`` with contiguous rows on 16-byte boundaries, and its row stride:
-    ``t`` itself, or a copy with padded rows (a base, width or stride that is no
-    multiple of 16 bytes)."""
-    unit = 16 // t.element_size()
+def _tma_rows(t: torch.Tensor, index: int, any_address: bool):
+    """2-D ``t`` with contiguous rows, and its row stride: ``t`` itself where its rows
+    lie on 16-byte boundaries (or need not), otherwise a copy with padded rows."""
+    size = t.element_size()
+    unit = 16 // size
     rows, n = t.shape
+    if n > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < n:
+        t = t.contiguous()
+    stride = t.stride(0) if rows > 1 else (n + unit - 1) // unit * unit
+    if any_address or t.data_ptr() % 16 == 0 and stride % unit == 0:
+        return t, stride
     wide = (n + unit - 1) // unit * unit
-    if t.data_ptr() % 16 == 0 and (t.stride(1) == 1 or n == 1):
-        if rows == 1:
-            return t, wide
-        if t.stride(0) % unit == 0 and t.stride(0) >= n:
-            return t, t.stride(0)
-    padded = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
-    padded[:, :n].copy_(t)
-    return padded, wide
+    packed = t.new_empty((rows, wide))
+    st = _native.load().b200_pack_rows(t.data_ptr(), stride * size, packed.data_ptr(), wide * size,
+                                       rows, n * size, _raw_stream(index))
+    if st:
+        _native.check(st, "b200_pack_rows")
+    return packed, wide
 
 
 def linear(x, weight, bias=None, activation=None, gated=False, residual=None, out=None,
@@ -999,8 +1002,8 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     too), and the result is act(gate) * up + residual.  ``activation``: None, "relu",
     "silu", "gelu" (error function) or "gelu_tanh".  bias: bf16; residual and
     ``out``: (..., n) bf16, ``out`` may be ``residual``.  Everything between the
-    operands and the one rounding at the end is fp32.  Operands whose rows do
-    not lie on 16-byte boundaries are copied to padded rows first.
+    operands and the one rounding at the end is fp32.  Above 8 tokens, operands
+    whose rows do not lie on 16-byte boundaries are copied to padded rows first.
     """
     assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
     dtype = x.dtype
@@ -1050,17 +1053,23 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
         y, y_stride = x.new_empty(shape, dtype=_BF16), n
     else:
         y, y_stride = out, max(n, _out_rows(out, shape, _BF16, index, "out").stride(0))
+    entry = _native.load().b200_linear
     unit = 16 if fp8 else 8
     if k % unit == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
         x2, x_stride, m = x, k, x.numel() // k
     else:
-        x2, x_stride = _tma_rows(_rows(x))
+        x2 = x if x.dim() == 2 else x.reshape(-1, k)
         m = x2.shape[0]
+        x2, x_stride = _tma_rows(x2, index, m <= 8)
+        if m <= 8:
+            entry = _native.load().b200_linear_unaligned
     if k % unit == 0 and weight.is_contiguous() and weight.data_ptr() % 16 == 0:
         w2, w_stride = weight, k
     else:
-        w2, w_stride = _tma_rows(weight)
-    st = _native.load().b200_linear(
+        w2, w_stride = _tma_rows(weight, index, m <= 8)
+        if m <= 8:
+            entry = _native.load().b200_linear_unaligned
+    st = entry(
         x2.data_ptr(), x_stride, xs_ptr, w2.data_ptr(), w_stride, ws_ptr, b_ptr, r_ptr, r_stride,
         y.data_ptr(), y_stride, m, n, k, fp8, gated, ACTIVATIONS[activation], _status_of(index),
         _raw_stream(index))

@@ -251,7 +251,8 @@ def test_product_epilogue(qb, act, m, k, n, gated, fp8):
 
 
 @pytest.mark.parametrize("how", ["padded", "odd"])
-@pytest.mark.parametrize("m,k,n", [(1, 96, 40), (4, 96, 41), (70, 513, 33), (140, 256, 64)])
+@pytest.mark.parametrize("m,k,n", [(1, 96, 40), (4, 96, 41), (70, 513, 33), (140, 256, 64), (8, 4999, 129),
+                                   (16, 333, 600), (9, 77, 17), (300, 1031, 257)])
 @pytest.mark.parametrize("fp8", [False, True])
 def test_product_strides(qb, how, m, k, n, fp8):
     a = _product(_gen(m + n), m, k, n, fp8, False, bias=True, residual=True, how=how)

@@ -85,3 +85,15 @@ def test_c_entry_refusals(native_lib):
     assert rot(q=None) == -1 and rot(hk=1) == -1
     assert lib.b200_rotary_tables(None, 0, 1, 0, fake, 1.0, fake, fake, 1, 1, 8, 0, None) == -1
     assert lib.b200_rotary_tables(fake, 0, 1, 0, fake, 1.0, None, fake, 1, 1, 8, 0, None) == -1
+
+
+def test_c_entry_refusals_of_unaligned_rows(native_lib):
+    lib = native_lib
+    few = lambda **k: lib.b200_linear_unaligned(*{**dict(  # noqa: E731
+        x=18, xs=65, sx=None, w=18, ws=65, sw=None, b=None, r=None, rs=0, o=16, os=8, m=1, n=8, k=65, fp8=0,
+        gated=0, act=0, dev=None, st=None), **k}.values())
+    assert few(m=0) == 0 and few(m=9) == -2 and few(k=0) == -1 and few(ws=64) == -1
+    pack = lambda **k: lib.b200_pack_rows(*{**dict(src=17, ss=33, dst=32, ds=48, rows=2, n=33, st=None),  # noqa: E731
+                                             **k}.values())
+    assert pack(rows=0) == 0 and pack(rows=-1) == -1 and pack(n=0) == -1 and pack(ds=47) == -1
+    assert pack(src=None) == -1 and pack(dst=40) == -3 and pack(ds=56) == -3
