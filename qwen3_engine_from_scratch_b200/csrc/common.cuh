@@ -329,24 +329,28 @@ B200_DEVICE float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 B200_DEVICE float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // 16 bytes from any address: the one or two aligned 16-byte words that hold them
-// (no byte outside the words that hold a wanted one is read), shifted into place.
-B200_DEVICE uint4 load_unaligned16(const void* p) {
+// (no byte outside the words that hold a wanted one is read), and the shift into
+// place, apart so that several loads can be under way.
+struct Unaligned16 {
+  uint4 a, b;
+  uint32_t off;
+};
+B200_DEVICE Unaligned16 load_unaligned16(const void* p) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p);
   const uint4* from = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
-  const uint32_t off = static_cast<uint32_t>(at & 15);
-  const uint4 a = from[0];
-  if (off == 0) return a;
-  const uint4 b = from[1];
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  if (off & 8) {
+  Unaligned16 u;
+  u.off = static_cast<uint32_t>(at & 15);
+  u.a = from[0];
+  u.b = from[u.off != 0 ? 1 : 0];
+  return u;
+}
+B200_DEVICE uint4 shifted(const Unaligned16& u) {
+  uint32_t w[8] = {u.a.x, u.a.y, u.a.z, u.a.w, u.b.x, u.b.y, u.b.z, u.b.w};
 #pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  }
-  if (off & 4) {
+  for (int i = 0; i < 6; ++i) w[i] = u.off & 8 ? w[i + 2] : w[i];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
-  const uint32_t bits = (off & 3) * 8;
+  for (int i = 0; i < 5; ++i) w[i] = u.off & 4 ? w[i + 1] : w[i];
+  const uint32_t bits = (u.off & 3) * 8;
   return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }

@@ -993,7 +993,7 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* src, int6
   const uint8_t* from = src + row * src_stride + at;
   uint4 v;
   if (at + 16 <= row_bytes) {
-    v = load_unaligned16(from);
+    v = shifted(load_unaligned16(from));
   } else {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll

@@ -6,7 +6,7 @@
 //   m16n8k16 (bf16) or m16n8k32 (e4m3): 16 weight rows x 8 tokens; a thread's four
 // words of a row's 16 bytes are the k pairs (quads) of two instructions.  Which
 // k an instruction sees at which place does not matter as long as W and X agree.
-// The 8 warps of a block split K of the block's rows and add their sums in warp
+// The 8 or 16 warps of a block split K of the block's rows and add their sums in warp
 // order through shared memory.  Gated: rows 0-7 of a tile are gate rows and rows
 // 8-15 the up rows of the same outputs.
 // Measured: 8 x 1024 x 4096 3.4 us in a graph, of which 1.3 are the weight's bytes;
@@ -17,8 +17,6 @@ namespace {
 
 using namespace b200;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;  // weight rows of a block
 constexpr int kStep = 64;  // bytes of K a warp takes of every row in a step
 
@@ -44,30 +42,46 @@ B200_DEVICE void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
   }
 }
 
+// 16 bytes of a row on their way
+template <bool ALIGNED>
+struct Piece {
+  uint4 w;
+};
+template <>
+struct Piece<false> {
+  Unaligned16 w;
+};
+B200_DEVICE uint4 value(const Piece<true>& p) { return p.w; }
+B200_DEVICE uint4 value(const Piece<false>& p) { return shifted(p.w); }
+
 // 16 bytes of a row from byte `at` on, zero past its end
 template <bool FP8, bool ALIGNED>
-B200_DEVICE uint4 piece(const uint8_t* row, int at, int end) {
-  if (at + 16 <= end)
-    return ALIGNED ? *reinterpret_cast<const uint4*>(row + at) : load_unaligned16(row + at);
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (at < end) {
-    uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-    for (int i = end - at - (FP8 ? 1 : 2); i >= 0; i -= FP8 ? 1 : 2) {  // the last element first
-      const uint64_t v = FP8 ? row[at + i] : *reinterpret_cast<const uint16_t*>(row + at + i);
-      constexpr int kBits = FP8 ? 8 : 16;
-      hi = (hi << kBits) | (lo >> (64 - kBits));
-      lo = (lo << kBits) | v;
-    }
-    w = make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32),
-                   static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
+B200_DEVICE Piece<ALIGNED> piece(const uint8_t* row, int at, int end) {
+  Piece<ALIGNED> p;
+  if (at + 16 <= end) {
+    if constexpr (ALIGNED) p.w = *reinterpret_cast<const uint4*>(row + at);
+    else p.w = load_unaligned16(row + at);
+    return p;
   }
-  return w;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (at < end) {
+#pragma unroll
+    for (int i = 0; i < 16; i += FP8 ? 1 : 2)
+      if (at + i < end) {
+        const uint32_t v = FP8 ? row[at + i] : *reinterpret_cast<const uint16_t*>(row + at + i);
+        w[i / 4] |= v << (8 * (i % 4));
+      }
+  }
+  const uint4 u = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (ALIGNED) p.w = u;
+  else p.w = Unaligned16{u, u, 0};
+  return p;
 }
 
 // TT token tiles of 8; a warp reads AHEAD steps before it multiplies the first
-template <int TT, int AHEAD, bool FP8, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs a) {
+template <int TT, int AHEAD, int WARPS, bool FP8, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS * 32) linear_small_kernel(const SmallArgs a) {
+  constexpr int kWarps = WARPS, kThreads = WARPS * 32;
   __shared__ float sums[kWarps][kRows][TT * 8 + 1];
   const LinearArgs& e = a.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -90,13 +104,13 @@ __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs 
   // (A prefetch returns no data: what that kernel still writes to W is read after
   // the wait, from L2 as always.)
   {
-    const int at = (threadIdx.x & 15) * 128;
-    if (at < a.k_bytes) prefetch_l2(weight_row(threadIdx.x >> 4) + at);
+    const int at = (threadIdx.x % (kThreads / kRows)) * 128;
+    if (at < a.k_bytes) prefetch_l2(weight_row(threadIdx.x / (kThreads / kRows)) + at);
   }
   pdl_begin();
   float d[TT][4] = {};
   for (int k0 = warp * kStep; k0 < a.k_bytes; k0 += kWarps * kStep * AHEAD) {
-    uint4 wv[AHEAD][2], xv[AHEAD][TT];
+    Piece<ALIGNED> wv[AHEAD][2], xv[AHEAD][TT];
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) {
       const int at = k0 + s * kWarps * kStep + t * 16;
@@ -106,13 +120,15 @@ __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs 
       for (int i = 0; i < TT; ++i) xv[s][i] = piece<FP8, ALIGNED>(x[i], at, a.k_bytes);
     }
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s)
+    for (int s = 0; s < AHEAD; ++s) {
+      const uint4 p = value(wv[s][0]), q = value(wv[s][1]);
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        const uint4 p = wv[s][0], q = wv[s][1], v = xv[s][i];
+        const uint4 v = value(xv[s][i]);
         mma<FP8>(d[i], p.x, q.x, p.y, q.y, v.x, v.y);
         mma<FP8>(d[i], p.z, q.z, p.w, q.w, v.z, v.w);
       }
+    }
   }
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
@@ -143,11 +159,11 @@ __global__ void __launch_bounds__(kThreads) linear_small_kernel(const SmallArgs 
   }
 }
 
-template <int TT, int AHEAD, bool ALIGNED>
+template <int TT, int AHEAD, int WARPS, bool ALIGNED>
 cudaError_t launch(const SmallArgs& a, bool fp8, unsigned blocks, cudaStream_t stream) {
-  return b200host::launch_pdl(fp8 ? linear_small_kernel<TT, AHEAD, true, ALIGNED>
-                                  : linear_small_kernel<TT, AHEAD, false, ALIGNED>,
-                              dim3(blocks), dim3(kThreads), 0, stream, a);
+  return b200host::launch_pdl(fp8 ? linear_small_kernel<TT, AHEAD, WARPS, true, ALIGNED>
+                                  : linear_small_kernel<TT, AHEAD, WARPS, false, ALIGNED>,
+                              dim3(blocks), dim3(WARPS * 32), 0, stream, a);
 }
 
 }  // namespace
@@ -176,16 +192,22 @@ cudaError_t linear_small(const b200::LinearArgs& e, const void* x, int64_t x_str
   const int tile_n = e.gated ? kRows / 2 : kRows;
   const unsigned blocks = static_cast<unsigned>((e.n + tile_n - 1) / tile_n);
   const bool aligned = aligned16(x) && aligned16(w) && a.x_row % 16 == 0 && a.w_row % 16 == 0;
-  if (!aligned)
-    return e.m > 8 ? launch<2, 4, false>(a, fp8, blocks, stream)
-                   : launch<1, 4, false>(a, fp8, blocks, stream);
-  if (e.m > 8) return launch<2, 4, true>(a, fp8, blocks, stream);
-  // Eight steps ahead where few blocks have to keep the memory busy and K feeds
-  // them: 8 x 4096 x 1024 6.3 -> 5.4 us, 8 x 12288 x 4096 23.3 -> 20.7; with more
-  // blocks than two an SM the registers cost more (8 x 4096 x 6144 10.7 -> 14.4).
-  if (blocks <= 2u * sms && a.k_bytes >= 8 * kWarps * kStep)
-    return launch<1, 8, true>(a, fp8, blocks, stream);
-  return launch<1, 4, true>(a, fp8, blocks, stream);
+  // 16 warps a block where there is about one block an SM, or less, and K feeds
+  // them: 8 x 4096 x 2048 6.3 -> 5.5 us, 1 x 2048 x 1024 3.2 -> 2.5; with two blocks an
+  // SM 8 warps are faster (8 x 4096 x 4096 8.5, 10.3 with 16).
+  const bool wide = blocks <= static_cast<unsigned>(sms) && a.k_bytes >= 8 * 8 * kStep;
+  if (!aligned) {
+    if (e.m > 8) return launch<2, 2, 8, false>(a, fp8, blocks, stream);
+    return wide ? launch<1, 2, 16, false>(a, fp8, blocks, stream)
+                : launch<1, 2, 8, false>(a, fp8, blocks, stream);
+  }
+  if (e.m > 8) return launch<2, 4, 8, true>(a, fp8, blocks, stream);
+  if (wide) return launch<1, 4, 16, true>(a, fp8, blocks, stream);
+  // Eight steps ahead with up to two blocks an SM: 8 x 12288 x 4096 23.3 -> 20.7; with
+  // more the registers cost more (8 x 4096 x 6144 10.7 -> 14.4).
+  if (blocks <= 2u * sms && a.k_bytes >= 8 * 8 * kStep)
+    return launch<1, 8, 8, true>(a, fp8, blocks, stream);
+  return launch<1, 4, 8, true>(a, fp8, blocks, stream);
 }
 
 }  // namespace b200host
