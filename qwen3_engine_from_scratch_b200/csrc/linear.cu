@@ -980,28 +980,38 @@ cudaError_t launch_bn(int bn, bool pair, const CUtensorMap& tw, const CUtensorMa
 
 namespace {
 
+constexpr int kPackAhead = 4;
+
 // dst rows (16-byte aligned, zero to the next multiple of 16 bytes) from src rows
-// at any address; a thread moves 16 bytes
+// at any address; a thread takes kPackAhead pieces of 16 bytes of a row
 __global__ void __launch_bounds__(256) pack_rows_kernel(const uint8_t* src, int64_t src_stride,
                                                         uint8_t* dst, int64_t dst_stride, int64_t rows,
-                                                        int row_bytes, int pieces) {
+                                                        int row_bytes) {
   pdl_begin();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = i / pieces;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (row >= rows) return;
-  const int at = static_cast<int>(i - row * pieces) * 16;
-  const uint8_t* from = src + row * src_stride + at;
-  uint4 v;
-  if (at + 16 <= row_bytes) {
-    v = shifted(load_unaligned16(from));
-  } else {
-    uint32_t w[4] = {0, 0, 0, 0};
+  const uint8_t* from = src + row * src_stride;
+  uint8_t* to = dst + row * dst_stride;
+  const int at0 = (blockIdx.y * blockDim.x * kPackAhead + threadIdx.x) * 16;
+  Unaligned16 u[kPackAhead];
 #pragma unroll
-    for (int b = 0; b < 15; ++b)
-      if (at + b < row_bytes) w[b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < kPackAhead; ++i) {
+    const int at = at0 + i * blockDim.x * 16;
+    if (at + 16 <= row_bytes) u[i] = load_unaligned16(from + at);
   }
-  *reinterpret_cast<uint4*>(dst + row * dst_stride + at) = v;
+#pragma unroll
+  for (int i = 0; i < kPackAhead; ++i) {
+    const int at = at0 + i * blockDim.x * 16;
+    if (at + 16 <= row_bytes) {
+      *reinterpret_cast<uint4*>(to + at) = shifted(u[i]);
+    } else if (at < row_bytes) {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < 15; ++b)
+        if (at + b < row_bytes) w[b >> 2] |= static_cast<uint32_t>(from[at + b]) << (8 * (b & 3));
+      *reinterpret_cast<uint4*>(to + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
 }
 
 }  // namespace
@@ -1013,12 +1023,17 @@ extern "C" int b200_pack_rows(const void* src, int64_t src_stride, void* dst, in
   const int pieces = (row_bytes + 15) / 16;
   if (!src || !dst || dst_stride < static_cast<int64_t>(pieces) * 16) return B200_ERR_INVALID_ARGUMENT;
   if (!b200host::aligned16(dst) || dst_stride % 16) return B200_ERR_ALIGNMENT;
-  const int64_t blocks = (rows * pieces + 255) / 256;
-  if (blocks > 0x7fffffff) return B200_ERR_INVALID_ARGUMENT;
+  int threads = (pieces + kPackAhead - 1) / kPackAhead;
+  threads = threads > 128 ? 256 : threads > 64 ? 128 : threads > 32 ? 64 : threads > 16 ? 32 : 16;
+  const int columns = (pieces + threads * kPackAhead - 1) / (threads * kPackAhead);
+  const int together = 256 / threads;  // rows of a block
+  const int64_t blocks = (rows + together - 1) / together;
+  if (blocks > 0x7fffffff || columns > 65535) return B200_ERR_INVALID_ARGUMENT;
   return b200host::status_from_cuda(b200host::launch_pdl(
-      pack_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
-      static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(src), src_stride,
-      static_cast<uint8_t*>(dst), dst_stride, rows, row_bytes, pieces));
+      pack_rows_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(columns)),
+      dim3(threads, together), 0, static_cast<cudaStream_t>(stream),
+      static_cast<const uint8_t*>(src), src_stride, static_cast<uint8_t*>(dst), dst_stride, rows,
+      row_bytes));
 }
 
 namespace {

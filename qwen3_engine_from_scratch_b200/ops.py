@@ -979,7 +979,8 @@ def _tma_rows(t: torch.Tensor, index: int, any_address: bool):
     stride = t.stride(0) if rows > 1 else (n + unit - 1) // unit * unit
     if any_address or t.data_ptr() % 16 == 0 and stride % unit == 0:
         return t, stride
-    wide = (n + unit - 1) // unit * unit
+    line = 128 // size                 # whole lines: a panel of a row then is one line, not two
+    wide = (n + line - 1) // line * line
     packed = t.new_empty((rows, wide))
     st = _native.load().b200_pack_rows(t.data_ptr(), stride * size, packed.data_ptr(), wide * size,
                                        rows, n * size, _raw_stream(index))
