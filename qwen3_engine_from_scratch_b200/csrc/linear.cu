@@ -849,11 +849,11 @@ int ensure_smem_attr(int dev) {
 // 128 bytes of K of a tile, or the weight's bytes at 5.6 TB/s where that is more,
 // and a third of the other (256 rows of 151,936 logits: 81 us in pairs of 256, 95
 // in (128), whose main loops alone would both hide behind the weight);
-// `epilogue` for the last tile's, `exchange` where K is split.  Over the 23
-// shapes the choice is within 3 % of the best cut on average and 15 % at most:
-// 64 x 12288 x 4096 in e4m3 takes 13.0 us in (64, split 4), 16.7 in (64, split 2),
-// 512 x 4096 x 4096 17.8 in pairs of 128, 18.9 in (128), 25 in (64) and 26 in
-// pairs of 256; 2048 x 1024 x 4096 16.6 in pairs of 256 and 19.1 in (128).
+// `epilogue` for the last tile's, `exchange` for each halving of K.  Over the 23
+// shapes the choice is within 2 % of the best cut on average and 10 % at most:
+// 64 x 12288 x 4096 in e4m3 takes 13.2 us in (64, split 4) and 16.8 in (64, split
+// 2), 512 x 4096 x 4096 18.0 in pairs of 128, 19.0 in (128) and 25 in (64) or
+// pairs of 256, 256 x 4096 x 4096 14.7 in (64) and 16.7 in (128, split 2).
 struct Cut {
   int bn;
   bool pair;
@@ -861,9 +861,9 @@ struct Cut {
   float panel, epilogue, exchange;
 };
 constexpr Cut kCuts[] = {
-    {32, false, 3, 0.16f, 0.1f, 0.0f},  {64, false, 3, 0.16f, 0.9f, 0.5f},
-    {128, false, 3, 0.225f, 1.3f, 1.8f}, {256, false, 0, 0.32f, 3.1f, 0.0f},
-    {128, true, 2, 0.15f, 3.0f, 1.3f},  {256, true, 0, 0.26f, 3.9f, 0.0f}};
+    {32, false, 3, 0.14f, 0.0f, 0.6f},   {64, false, 3, 0.146f, 0.1f, 0.62f},
+    {128, false, 3, 0.206f, 0.4f, 3.0f}, {256, false, 0, 0.31f, 1.2f, 0.0f},
+    {128, true, 2, 0.15f, 1.6f, 3.1f},   {256, true, 0, 0.25f, 2.1f, 0.0f}};
 
 struct Plan {
   int bn, splits;
@@ -888,7 +888,7 @@ Plan choose(int m, int n_tiles, int k_panels, const int* resident) {
       if (splits > 1 && waves > 1.0f) break;  // clusters that split K do not persist
       const float main = waves * ((k_panels + splits - 1) / splits) * c.panel;
       const float t = 4.0f + (main > read ? main + 0.35f * read : read + 0.35f * main) +
-                      c.epilogue + (splits > 1 ? c.exchange : 0.0f);
+                      c.epilogue + log * c.exchange;
       if (t < least) {
         least = t;
         best = Plan{c.bn, splits, c.pair};
