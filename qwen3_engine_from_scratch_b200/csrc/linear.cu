@@ -7,8 +7,8 @@
 //
 // The weight's rows are the M side of the instruction (128 TMEM lanes) and the
 // tokens its N side: a decode step of a few tokens then streams W through full
-// 128-row tiles and pads only the small token side, and one kernel serves one
-// token and thousands.  Token tiles of BN columns; two accumulators of BN
+// 128-row tiles and pads only the small token side, and one kernel serves nine
+// tokens and thousands.  Token tiles of BN columns; two accumulators of BN
 // columns, so the epilogue of one tile overlaps the product of the next.
 //   warps 0-15   epilogue: lane l of warp w owns accumulator lane 32 (w % 4) + l,
 //                of every fourth 16 token columns
@@ -27,15 +27,15 @@
 // Few tiles (a decode step): the CTAs (or pairs) of a cluster share one tile and
 // split K; every CTA sends its fp32 partial to the CTA that owns its token columns
 // through distributed shared memory, and the owners add the partials in rank
-// order, so the result does not depend on timing.  Up to 16 tokens go to the
-// direct kernel of linear_small.cu.
+// order, so the result does not depend on timing.  Up to 8 tokens (16 with a small
+// weight) go to the direct kernel of linear_small.cu.
 //
 // Bounds and what it measured (B200): large products by the tensor pipe, 95 %
 // active in bf16 and 91 % in e4m3 at the 1.5 GHz that the power cap leaves: 4096
-// tokens, 4096 -> 2 x 12288 gated with silu in 586 us (1.41 PFLOP/s) and 316 us
+// tokens, 4096 -> 2 x 12288 gated with silu in 570 us (1.45 PFLOP/s) and 316 us
 // (2.61 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
-// of tiles: 81 us (4.8 TB/s).  64 x 12288 x 4096 in e4m3 by the weight's bytes and about 5 us
-// of launch, first loads, exchange and end: 12.4 us (4.2 TB/s).
+// of tiles: 83 us (4.7 TB/s).  64 x 12288 x 4096 in e4m3 by the weight's bytes and about 5 us
+// of launch, first loads, exchange and end: 12.7 us (4.1 TB/s).
 //
 // Every wait is bounded: one that runs out sets B200_DEV_TIMEOUT, the other
 // roles give up too, outstanding copies are awaited and TMEM is freed.
