@@ -845,7 +845,7 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh":
 # Single calls of these operators are bound by the host (a launch is about 3 of 11
 # us), so their checks use the cheap accessors.
 
-_BF16, _F32 = torch.bfloat16, torch.float32
+_BF16, _F32, _CONTIGUOUS = torch.bfloat16, torch.float32, torch.contiguous_format
 _current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -904,12 +904,11 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
     y_stride = hidden
     if out is not None:
         y, y_stride = out, _out_rows(out, shape, FP8 if fp8 else _BF16, index, "out").stride(0)
-    elif fp8:
-        y = x.new_empty(shape, dtype=FP8)
     else:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = torch.empty_like(x, dtype=FP8 if fp8 else _BF16, memory_format=_CONTIGUOUS)
     if fp8:
-        scale = x.new_empty(shape[:-1], dtype=_F32)
+        scale = torch.empty_strided((rows,), (1,), dtype=_F32, device=x.device) \
+            if len(shape) == 2 else x.new_empty(shape[:-1], dtype=_F32)
         s_ptr = scale.data_ptr()
     if residual is not None:
         assert residual.dtype is _BF16 and residual.shape == shape, \
@@ -922,7 +921,7 @@ def _norm(x, weight, residual, eps, fp8, out, residual_out, what):
             r_stride = r2.stride(0)
         r_ptr, h_stride = r2.data_ptr(), hidden
         if residual_out is None:
-            h = torch.empty_like(x, memory_format=torch.contiguous_format)
+            h = torch.empty_like(x, memory_format=_CONTIGUOUS)
         else:
             h, h_stride = residual_out, _out_rows(residual_out, shape, _BF16, index,
                                                   "residual_out").stride(0)
@@ -1051,7 +1050,9 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
             r_stride = max(n, r2.stride(0))
         r_ptr = r2.data_ptr()
     if out is None:
-        y, y_stride = x.new_empty(shape, dtype=_BF16), n
+        y = torch.empty_strided(shape, (n, 1), dtype=_BF16, device=x.device) \
+            if len(shape) == 2 else x.new_empty(shape, dtype=_BF16)
+        y_stride = n
     else:
         y, y_stride = out, max(n, _out_rows(out, shape, _BF16, index, "out").stride(0))
     entry = _native.load().b200_linear

@@ -320,6 +320,21 @@ def test_product_leading_dimensions_streams_and_graph(qb):
     assert torch.equal(out, flat)
 
 
+def test_product_waits_for_the_host_after_a_timeout(qb):
+    """With a timeout on record the pipelined product starts nothing; cleared, it works."""
+    a = _product(_gen(1), 100, 256, 256)
+    want = qb.linear(**a)
+    out = torch.full_like(want, 3.0)
+    qb.ops._status[torch.cuda.current_device()].fill_(0x10)       # B200_DEV_TIMEOUT
+    qb.linear(out=out, **a)
+    with pytest.raises(RuntimeError, match="timed out"):
+        qb.check_device_status()
+    assert (out == 3.0).all()
+    qb.clear_device_status()
+    assert torch.equal(qb.linear(out=out, **a), want)
+    qb.check_device_status()
+
+
 def test_product_empty_and_refusals(qb):
     x = torch.ones(2, 32, dtype=BF16, device="cuda")
     w = torch.ones(6, 32, dtype=BF16, device="cuda")
