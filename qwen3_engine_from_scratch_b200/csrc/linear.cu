@@ -54,6 +54,7 @@ constexpr int kAPanel = kRows * kKBytes;
 constexpr int kEpilogueWarps = 16;
 constexpr int kSides = kEpilogueWarps / 4;  // warps of a lane quarter
 constexpr int kCols = 16;                   // columns they take in turn
+static_assert(kSides * kCols >= 64, "the columns a CTA owns at most in a split product");
 constexpr int kThreads = (kEpilogueWarps + 3) * 32;
 constexpr int kScales = (256 + kSides * kCols - 1) / (kSides * kCols) * kCols;  // of a warp
 constexpr int kWeightWarp = kEpilogueWarps;
@@ -509,35 +510,30 @@ struct Epilogue {
   }
 };
 
-// The columns of this CTA in a split product, N at a time: the partials of all
-// ranks in rank order, then the epilogue.
+// N of the columns of this CTA in a split product: the partials of all ranks in
+// rank order, then the epilogue.  The warps of a lane quarter share the columns
+// (kSides N of them, at least as many as a CTA owns).
 template <int N>
 B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t exchange, int own,
-                              int token0, int warp, int lane, float* xs) {
+                              int token0, int warp, int lane, const float* xs) {
   const int row = (warp & 3) * 32 + lane;
-#pragma unroll 1
-  for (int c = (warp >> 2) * N; c < own && token0 + c < a.m; c += kSides * N) {
-    if (a.w_scale != nullptr) {
-      __syncwarp();
-      if (lane < N) xs[lane] = token0 + c + lane < a.m ? a.x_scale[token0 + c + lane] : 0.0f;
-      __syncwarp();
-    }
-    float v[N];
+  const int c = (warp >> 2) * N;
+  if (c >= own || token0 + c >= a.m) return;
+  float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
 #pragma unroll 2
-    for (int from = 0; from < a.splits; ++from) {
+  for (int from = 0; from < a.splits; ++from) {
 #pragma unroll
-      for (int i = 0; i < N; i += 4) {
-        const float4 p = ld_shared(exchange + exchange_at(from, row, own, (c + i) >> 2));
-        v[i] += p.x;
-        v[i + 1] += p.y;
-        v[i + 2] += p.z;
-        v[i + 3] += p.w;
-      }
+    for (int i = 0; i < N; i += 4) {
+      const float4 p = ld_shared(exchange + exchange_at(from, row, own, (c + i) >> 2));
+      v[i] += p.x;
+      v[i + 1] += p.y;
+      v[i + 2] += p.z;
+      v[i + 3] += p.w;
     }
-    ep.put_columns<N>(token0 + c, v, xs, [] {});
   }
+  ep.put_columns<N>(token0 + c, v, xs, [] {});
 }
 
 template <int BN, bool FP8, bool PAIR>
@@ -630,7 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = first; ok && tile < tiles; tile += stride) {
       const Tile t = tile == first ? first_tile : tile_at<BN, PAIR>(a, tile, half);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = warp_wait(empty(stage), phase ^ 1, &B, a.dev_status))) break;
+        // (the first use of a stage finds it empty: no wait on the launch's path)
+        if (issued >= a.stages && !(ok = warp_wait(empty(stage), phase ^ 1, &B, a.dev_status)))
+          break;
         if (elected) {
           // PAIR: both CTAs' copies count on the first CTA's barrier
           const uint32_t bar = PAIR ? remote_smem(full(stage), leader) : full(stage);
@@ -770,14 +768,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   __syncwarp();
   if (a.splits > 1) {  // one tile a cluster
+    const bool finishes = warp < kEpilogueWarps && first < tiles;
+    const int own = BN / a.splits;
+    const int token0 = first_tile.token0 + part * own;
+    const int at_once = own >= 32 ? 16 : own >= 16 ? 8 : 4;
+    // scales and bias come while the partials travel
+    const Epilogue ep(a, first_tile.n0, warp, lane, turn[finishes ? warp : 0]);
+    if (finishes && a.w_scale != nullptr && lane < at_once) {
+      const int t = token0 + (warp >> 2) * at_once + lane;
+      xs[warp][lane] = t < a.m ? a.x_scale[t] : 0.0f;
+    }
     cluster_sync();
-    if (warp < kEpilogueWarps && first < tiles && B.error == 0) {
-      const int own = BN / a.splits;
-      const int token0 = first_tile.token0 + part * own;
-      const Epilogue ep(a, first_tile.n0, warp, lane, turn[warp]);
-      // the warps of a lane quarter share the columns
-      if (own >= 32) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
-      else if (own == 16) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+    if (finishes && B.error == 0) {
+      if (at_once == 16) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      else if (at_once == 8) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
       else finish_split<4>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
     }
   }
