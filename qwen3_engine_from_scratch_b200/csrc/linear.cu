@@ -866,7 +866,7 @@ struct Cut {
 };
 constexpr Cut kCuts[] = {
     {32, false, 3, 0.14f, 0.0f, 0.6f},   {64, false, 3, 0.146f, 0.1f, 0.62f},
-    {128, false, 3, 0.206f, 0.4f, 3.0f}, {256, false, 0, 0.31f, 1.2f, 0.0f},
+    {128, false, 2, 0.206f, 0.4f, 3.0f}, {256, false, 0, 0.31f, 1.2f, 0.0f},
     {128, true, 2, 0.15f, 1.6f, 3.1f},   {256, true, 0, 0.25f, 2.1f, 0.0f}};
 
 struct Plan {

@@ -241,6 +241,20 @@ def test_product_sizes(qb, m, k, n, fp8, gated):
     _check_product(qb.linear(activation=act, gated=gated, **a), a, act, gated)
 
 
+@pytest.mark.parametrize("m,k,n", [(25, 6208, 80256), (49, 1216, 3456), (22, 4800, 1536), (240, 11712, 128),
+                                   (3202, 896, 128), (123, 11520, 1152), (42, 23680, 1536), (7854, 8640, 128),
+                                   (252, 19008, 2176), (1364, 64, 51328), (200, 22656, 4352), (1247, 20608, 256),
+                                   (1627, 832, 2176), (1300, 2944, 8704)])
+def test_product_cuts(qb, m, k, n):
+    """A shape for every cut the cost model takes: tiles of 32 to 256 tokens, K split
+    2 to 8 ways, pairs of CTAs with and without a split."""
+    a = _product(_gen(m + n), m, k, n, residual=True)
+    got = qb.linear(activation="silu", **a)
+    at = torch.arange(0, n, max(1, n // 2500), device="cuda")        # the reference: some columns of the wide ones
+    part = dict(a, weight=a["weight"][at], residual=a["residual"][:, at])
+    _check_product(got[:, at], part, "silu", False)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("m,k,n", [(3, 256, 160), (150, 200, 99), (600, 128, 512)])
 @pytest.mark.parametrize("gated", [False, True])
