@@ -308,6 +308,11 @@ struct Epilogue {
     bias = a.bias != nullptr && live ? __bfloat162float(a.bias[w_row]) : 0.0f;
   }
 
+  // the line that holds this warp's columns of a token
+  B200_DEVICE void prefetch_residual(int token) const {
+    if (base_n < a.n) prefetch_l2(a.residual + token * a.r_row + base_n);
+  }
+
   // Any strides: v[i] is the output of column row_n and token + i * step.
   template <int M>
   B200_DEVICE void put_direct(int token, int step, float (&v)[M]) const {
@@ -337,14 +342,14 @@ struct Epilogue {
   struct Piece {
     uint4 even, odd;
   };
-  B200_DEVICE void fetch(int token, Piece& p) const {
+  B200_DEVICE void fetch_plain(int token, Piece& p) const {
     const int t = token + (lane >> 2) * 2, n = base_n + (lane & 3) * 8;
     p.even = p.odd = make_uint4(0, 0, 0, 0);
     const __nv_bfloat16* r = a.residual + t * a.r_row + n;
     if (n < a.n && t < a.m) p.even = *reinterpret_cast<const uint4*>(r);
     if (n < a.n && t + 1 < a.m) p.odd = *reinterpret_cast<const uint4*>(r + a.r_row);
   }
-  B200_DEVICE void put_plain(int token, float (&v)[16], const Piece& res) const {
+  B200_DEVICE void put_plain(int token, float (&v)[16], Piece& res, int next) const {
     const int pair = lane >> 2, unit = (lane & 3) * 2;
     if (a.residual != nullptr) {
       *unit_at(pair, unit) =
@@ -354,6 +359,7 @@ struct Epilogue {
           make_uint4(even_halves(res.even.z, res.odd.z), odd_halves(res.even.z, res.odd.z),
                      even_halves(res.even.w, res.odd.w), odd_halves(res.even.w, res.odd.w));
       __syncwarp();
+      if (next >= 0) fetch_plain(next, res);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t w = *word_at(i);
@@ -390,12 +396,13 @@ struct Epilogue {
     p.even = make_uint4(even_halves(x.x, y.x), odd_halves(x.x, y.x), even_halves(x.y, y.y),
                         odd_halves(x.y, y.y));
   }
-  B200_DEVICE void put_gated(int token, float (&v)[8], const Piece& res) const {
+  B200_DEVICE void put_gated(int token, float (&v)[8], Piece& res, int next) const {
     uint32_t* mine = buf + (high ? 16 : 0) + (lane & 15);  // + 32 a row pair
     uint4* piece = reinterpret_cast<uint4*>(buf) + lane;
     if (a.residual != nullptr) {
       *piece = res.even;
       __syncwarp();
+      if (next >= 0) fetch_gated(next, res);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[2 * i] += bf16_lo(mine[32 * i]);
@@ -458,17 +465,19 @@ struct Epilogue {
     }
   }
 
-  // accumulators of the tokens token .. token + N - 1; xs: their scales; `wait`
-  // ends when they are there
+  // This lane's words of the residual of 16 tokens, where put_columns<16> wants them.
+  B200_DEVICE void fetch(int token, Piece& p) const {
+    if (!a.wide || a.residual == nullptr) return;
+    if (a.gated) fetch_gated(token, p);
+    else fetch_plain(token, p);
+  }
+
+  // accumulators of the tokens token .. token + N - 1; xs: their scales; res: what
+  // fetch() gave for them, and gives for `next` (if any) when it is free; `wait`
+  // ends when the accumulators are there
   template <int N, class Wait>
-  B200_DEVICE void put_columns(int token, float (&v)[N], const float* xs, Wait&& wait) const {
-    Piece res;
-    if constexpr (N == 16) {
-      if (a.wide && a.residual != nullptr) {  // read while the accumulators come
-        if (a.gated) fetch_gated(token, res);
-        else fetch(token, res);
-      }
-    }
+  B200_DEVICE void put_columns(int token, float (&v)[N], const float* xs, Piece& res, int next,
+                               Wait&& wait) const {
     wait();
     if (a.w_scale != nullptr) {
 #pragma unroll
@@ -492,7 +501,7 @@ struct Epilogue {
       for (int i = 0; i < N / 2; ++i) gate[i] *= up[i];
       if constexpr (N == 16) {
         if (a.wide) {
-          put_gated(token, gate, res);
+          put_gated(token, gate, res, next);
           return;
         }
       }
@@ -501,7 +510,7 @@ struct Epilogue {
       activate(v, a.act);
       if constexpr (N == 16) {
         if (a.wide) {
-          put_plain(token, v, res);
+          put_plain(token, v, res, next);
           return;
         }
       }
@@ -515,7 +524,8 @@ struct Epilogue {
 // (kSides N of them, at least as many as a CTA owns).
 template <int N>
 B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t exchange, int own,
-                              int token0, int warp, int lane, const float* xs) {
+                              int token0, int warp, int lane, const float* xs,
+                              Epilogue::Piece& res) {
   const int row = (warp & 3) * 32 + lane;
   const int c = (warp >> 2) * N;
   if (c >= own || token0 + c >= a.m) return;
@@ -533,7 +543,7 @@ B200_DEVICE void finish_split(const LinearArgs& a, const Epilogue& ep, uint32_t 
       v[i + 3] += p.w;
     }
   }
-  ep.put_columns<N>(token0 + c, v, xs, [] {});
+  ep.put_columns<N>(token0 + c, v, xs, res, -1, [] {});
 }
 
 template <int BN, bool FP8, bool PAIR>
@@ -733,6 +743,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
+      if (a.residual != nullptr) {  // its lines come to L2 while the product runs
+        const int from = a.splits == 1 ? 0 : part * (BN / a.splits);
+        const int to = a.splits == 1 ? cols : min(cols, from + BN / a.splits);
+        for (int c = from + side * 32 + lane; c < to; c += kSides * 32) ep.prefetch_residual(t.token0 + c);
+      }
+      Epilogue::Piece res;
+      if (a.splits == 1 && side * kCols < cols) ep.fetch(t.token0 + side * kCols, res);
       if (!warp_wait(acc_full(buf), (count >> 1) & 1, &B, a.dev_status)) break;
       tc_fence_after();
       if (a.splits == 1) {
@@ -740,7 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = side * kCols, j = 0; c < cols; c += kTurn, j += kCols) {
           float v[kCols];
           tmem_ld16(acc + c, reinterpret_cast<uint32_t*>(v));
-          ep.put_columns<kCols>(t.token0 + c, v, &xs[warp][j],
+          ep.put_columns<kCols>(t.token0 + c, v, &xs[warp][j], res,
+                                c + kTurn < cols ? t.token0 + c + kTurn : -1,
                                 [&] { tmem_wait_ld16(reinterpret_cast<uint32_t*>(v)); });
         }
         tc_fence_before();
@@ -771,18 +789,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool finishes = warp < kEpilogueWarps && first < tiles;
     const int own = BN / a.splits;
     const int token0 = first_tile.token0 + part * own;
-    const int at_once = own >= 32 ? 16 : own >= 16 ? 8 : 4;
+    const int at_once = own >= 32 || (own == 16 && a.wide) ? 16 : own >= 16 ? 8 : 4;
     // scales and bias come while the partials travel
     const Epilogue ep(a, first_tile.n0, warp, lane, turn[finishes ? warp : 0]);
     if (finishes && a.w_scale != nullptr && lane < at_once) {
       const int t = token0 + (warp >> 2) * at_once + lane;
       xs[warp][lane] = t < a.m ? a.x_scale[t] : 0.0f;
     }
+    Epilogue::Piece res;
+    if (finishes && at_once == 16) ep.fetch(token0 + (warp >> 2) * 16, res);
     cluster_sync();
     if (finishes && B.error == 0) {
-      if (at_once == 16) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
-      else if (at_once == 8) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
-      else finish_split<4>(a, ep, exchange, own, token0, warp, lane, xs[warp]);
+      if (at_once == 16) finish_split<16>(a, ep, exchange, own, token0, warp, lane, xs[warp], res);
+      else if (at_once == 8) finish_split<8>(a, ep, exchange, own, token0, warp, lane, xs[warp], res);
+      else finish_split<4>(a, ep, exchange, own, token0, warp, lane, xs[warp], res);
     }
   }
   tc_fence_before();
