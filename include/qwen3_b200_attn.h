@@ -461,6 +461,18 @@ int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q
                 int num_heads, int num_kv_heads, int head_dim, int rotary_dim, int interleaved,
                 void* stream);
 
+/*
+ * b200_rms_norm (15 words), b200_linear (19 words, then 1 for the rules of
+ * b200_linear_unaligned or 0) and b200_rotary (30 words) with their arguments in
+ * one array, a 64-bit word each, in the same order: pointers, strides, sizes and
+ * flags as integers, eps and gain as doubles.  A binding passes one pointer where
+ * converting each argument costs more than the call; a size or flag that does not
+ * fit an int is refused (B200_ERR_INVALID_ARGUMENT).
+ */
+int b200_rms_norm_words(const int64_t* words);
+int b200_linear_words(const int64_t* words);
+int b200_rotary_words(const int64_t* words);
+
 /* cos and sin rows (batch, seq, rotary_dim) fp32, contiguous, of the same plan:
  * what b200_qk_norm_rope_kv_write takes (half layout). */
 int b200_rotary_tables(const void* positions, int64_t pos_stride_b, int64_t pos_stride_s,

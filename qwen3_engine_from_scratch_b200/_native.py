@@ -99,6 +99,9 @@ SIGNATURES = {
     "b200_rotary": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                          _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                          _P, _I64, _I64, _I, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "b200_rms_norm_words": (_I, [ctypes.c_char_p]),
+    "b200_linear_words": (_I, [ctypes.c_char_p]),
+    "b200_rotary_words": (_I, [ctypes.c_char_p]),
     "b200_rotary_tables": (_I, [_P, _I64, _I64, _I, _P, _F, _P, _P, _I, _I, _I, _I, _P]),
 }
 

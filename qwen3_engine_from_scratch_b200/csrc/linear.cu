@@ -43,6 +43,7 @@
 
 #include "linear.cuh"
 #include "tcgen05.cuh"
+#include "words.cuh"
 
 namespace {
 
@@ -1150,4 +1151,17 @@ extern "C" int b200_linear_unaligned(const void* x, int64_t x_stride, const floa
   if (m > 8) return B200_ERR_UNSUPPORTED;
   return linear_any(x, x_stride, x_scale, w, w_stride, w_scale, bias, residual, r_stride, out,
                     o_stride, m, n, k, fp8, gated, activation, dev_status, stream, true);
+}
+
+extern "C" int b200_linear_words(const int64_t* words) {
+  if (!words) return B200_ERR_INVALID_ARGUMENT;
+  b200host::Words w{words};
+  const int m = w.integer(11), n = w.integer(12), k = w.integer(13);
+  const int fp8 = w.integer(14), gated = w.integer(15), activation = w.integer(16);
+  const bool any_address = w.integer(19) != 0;
+  if (!w.fit) return B200_ERR_INVALID_ARGUMENT;
+  const auto entry = any_address ? b200_linear_unaligned : b200_linear;
+  return entry(w.pointer(0), w.wide(1), w.pointer<float>(2), w.pointer(3), w.wide(4),
+               w.pointer<float>(5), w.pointer(6), w.pointer(7), w.wide(8), w.pointer(9), w.wide(10),
+               m, n, k, fp8, gated, activation, w.pointer<int32_t>(17), w.pointer(18));
 }

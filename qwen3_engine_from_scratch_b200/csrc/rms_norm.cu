@@ -23,6 +23,7 @@
 // rate), to bf16 44 us (0.93); 8192 x 12288 to e4m3 without a norm 48.3 us (0.95); one
 // row of 1024 1.5 us in a graph, its latency.
 #include "common.cuh"
+#include "words.cuh"
 
 #include <cuda_fp8.h>
 
@@ -554,4 +555,14 @@ extern "C" int b200_rms_norm(const void* x, int64_t x_stride, const void* residu
             : vec ? launch_held<8, 4>(a, grid, block, cs) : launch_held<1, 8>(a, grid, block, cs);
   }
   return b200host::status_from_cuda(e);
+}
+
+extern "C" int b200_rms_norm_words(const int64_t* words) {
+  if (!words) return B200_ERR_INVALID_ARGUMENT;
+  b200host::Words w{words};
+  const int hidden = w.integer(11);
+  if (!w.fit) return B200_ERR_INVALID_ARGUMENT;
+  return b200_rms_norm(w.pointer(0), w.wide(1), w.pointer(2), w.wide(3), w.pointer(4), w.pointer(5),
+                       w.wide(6), w.pointer<float>(7), w.pointer(8), w.wide(9), w.wide(10), hidden,
+                       w.real(12), w.pointer<int32_t>(13), w.pointer(14));
 }

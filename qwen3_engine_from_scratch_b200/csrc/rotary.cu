@@ -15,6 +15,7 @@
 // memory, then its threads (16 elements of a head each: 8 pairs, or 16 copied
 // elements; neighbours in a head, then in heads) walk over the tokens' heads.
 #include "common.cuh"
+#include "words.cuh"
 
 namespace {
 
@@ -319,4 +320,18 @@ extern "C" int b200_rotary_tables(const void* positions, int64_t pos_stride_b,
                                              dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                                              static_cast<cudaStream_t>(stream), a, cos_out, sin_out);
   return b200host::status_from_cuda(e);
+}
+
+extern "C" int b200_rotary_words(const int64_t* words) {
+  if (!words) return B200_ERR_INVALID_ARGUMENT;
+  b200host::Words w{words};
+  const int wide_positions = w.integer(19), batch = w.integer(22), seq = w.integer(23);
+  const int heads = w.integer(24), kv_heads = w.integer(25), dim = w.integer(26);
+  const int rotary_dim = w.integer(27), interleaved = w.integer(28);
+  if (!w.fit) return B200_ERR_INVALID_ARGUMENT;
+  return b200_rotary(w.pointer(0), w.wide(1), w.wide(2), w.wide(3), w.pointer(4), w.wide(5),
+                     w.wide(6), w.wide(7), w.pointer(8), w.wide(9), w.wide(10), w.wide(11),
+                     w.pointer(12), w.wide(13), w.wide(14), w.wide(15), w.pointer(16), w.wide(17),
+                     w.wide(18), wide_positions, w.pointer<uint64_t>(20), w.real(21), batch, seq,
+                     heads, kv_heads, dim, rotary_dim, interleaved, w.pointer(29));
 }

@@ -487,3 +487,12 @@ def test_rotary_empty_and_refusals(qb):
                 lambda: qb.rotary(q, None, p, plan, q_out=q[:2])):
         with pytest.raises(AssertionError):
             bad()
+
+
+def test_sizes_past_31_bits_are_refused(qb):
+    """Not cut to their low 32 bits, which would be 8 here."""
+    x = torch.empty(1, 2**32 + 8, dtype=BF16, device="cuda")
+    with pytest.raises(RuntimeError):
+        qb.quantize_rows_fp8(x)
+    with pytest.raises(RuntimeError):
+        qb.linear(x, x)

@@ -97,3 +97,29 @@ def test_c_entry_refusals_of_unaligned_rows(native_lib):
                                              **k}.values())
     assert pack(rows=0) == 0 and pack(rows=-1) == -1 and pack(n=0) == -1 and pack(ds=47) == -1
     assert pack(src=None) == -1 and pack(dst=40) == -3 and pack(ds=56) == -3
+
+
+def test_c_entries_of_packed_words(native_lib):
+    """One array of 64-bit words: the same refusals, and sizes past 31 bits are not cut."""
+    import struct
+    over, fake = 2**32 + 8, 16
+    call = lambda name, form, words: getattr(native_lib, name)(struct.pack(form, *words))  # noqa: E731
+    norm = [fake, 8, 0, 0, fake, fake, 8, 0, 0, 0, 1, 8, 1e-6, 0, 0]
+    lin = [fake, 64, 0, fake, 64, 0, 0, 0, 0, fake, 8, 1, 8, 64, 0, 0, 0, 0, 0, 0]
+    rot = [fake, 8, 8, 8, 0, 0, 0, 0, fake, 8, 8, 8, 0, 0, 0, 0, fake, 0, 1, 0, fake, 1.0, 1, 1, 1, 0, 8, 8, 0, 0]
+    for name, form, words, changes in (
+            ("b200_rms_norm_words", "12qd2q", norm,
+             [(10, 0, 0), (10, -1, -1), (0, 0, -1), (2, fake, -1), (4, 0, -1), (11, over, -1), (11, -8, -1)]),
+            ("b200_linear_words", "20q", lin,
+             [(11, 0, 0), (11, -1, -1), (11, over, -1), (12, over, -1), (13, over, -1), (16, 5, -1), (14, 1, -1),
+              (2, fake, -1), (10, 7, -1), (0, 18, -3), (4, 68, -3)]),
+            ("b200_rotary_words", "21qd8q", rot,
+             [(23, 0, 0), (24, 0, 0), (27, 7, -1), (22, -1, -1), (16, 0, -1), (25, 1, -1), (22, over, -1),
+              (23, over, -1), (24, over, -1), (26, over, -1), (27, over, -1)])):
+        assert getattr(native_lib, name)(None) == -1
+        for place, value, status in changes:
+            changed = list(words)
+            changed[place] = value
+            assert call(name, form, changed) == status, (name, place, value)
+    lin[19], lin[11] = 1, 9
+    assert call("b200_linear_words", "20q", lin) == -2
