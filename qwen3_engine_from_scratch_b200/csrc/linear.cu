@@ -32,10 +32,11 @@
 //
 // Bounds and what it measured (B200): large products by the tensor pipe, 95 %
 // active in bf16 and 91 % in e4m3 at the 1.5 GHz that the power cap leaves: 4096
-// tokens, 4096 -> 2 x 12288 gated with silu in 570 us (1.45 PFLOP/s) and 316 us
-// (2.61 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
-// of tiles: 83 us (4.7 TB/s).  64 x 12288 x 4096 in e4m3 by the weight's bytes and about 5 us
-// of launch, first loads, exchange and end: 12.7 us (4.1 TB/s).
+// tokens, 4096 -> 2 x 12288 gated with silu in 584 us (1.41 PFLOP/s) and 319 us
+// (2.59 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
+// of tiles: 90 us (4.3 TB/s; 81 into one output that partly stays in L2).  64 x 12288 x
+// 4096 in e4m3 by the weight's bytes and about 5 us of launch, first loads, exchange
+// and end: 12.8 us (4.0 TB/s), 13.7 with a residual.
 //
 // Every wait is bounded: one that runs out sets B200_DEV_TIMEOUT, the other
 // roles give up too, outstanding copies are awaited and TMEM is freed.
