@@ -14,7 +14,8 @@ the whole decoder layer runs on the package's kernels: ``rms_norm`` (with the
 residual's addition before the MLP), ``linear`` (the gated activation and the
 second residual in its epilogue) and, in 8 bits, ``rms_norm_fp8`` and
 ``quantize_rows_fp8`` in front of each product.  ``rope_plan`` scales the rotary
-frequencies for long contexts; ``qk_norm=False`` turns q and k by ``rotary``.
+frequencies for long contexts (with the QK norm it turns the whole head in the
+half layout); ``qk_norm=False`` turns q and k by ``rotary`` and any plan.
 The attention path is this package's in every case:
 
 * prefill (packed tokens of all requests): ``qk_norm_rope_kv_write`` (QK norm
@@ -56,6 +57,11 @@ class Qwen3DecodeModel:
                  intermediate=3072, vocab=151936, rope_theta=1e6, eps=1e-6, max_pos=4096,
                  seed=0, std=0.02, layer_ops="torch", rope_plan=None, qk_norm=True):
         assert layer_ops in ("torch", "bf16", "fp8"), "layer_ops must be torch, bf16 or fp8"
+        if rope_plan is not None and qk_norm:      # by tables, which do not tell their layout
+            assert not rope_plan.interleaved and rope_plan.rotary_dim == head_dim, \
+                "with qk_norm a rope_plan must turn the whole head in the half layout"
+        assert rope_plan is None or rope_plan.rotary_dim <= head_dim, \
+            "the rope_plan's rotary_dim exceeds head_dim"
         g = torch.Generator(device=device).manual_seed(seed)
         bf = torch.bfloat16
 
