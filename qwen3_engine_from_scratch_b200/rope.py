@@ -12,11 +12,15 @@ i of ``rotary_dim`` elements turns by f_i = base^(-2i / rotary_dim) a position
 ``bands``   by the turns n_i = original_len f_i / 2 pi a pair makes over the
             trained range: at most ``slow_turns``, f_i / factor; at least
             ``fast_turns``, f_i; between, the two mixed linearly in n_i.
-``yarn``    as bands, but mixed linearly in the pair's index between the
-            (whole) indices at which a pair makes ``fast_turns`` and
-            ``slow_turns``; cos and sin are scaled by 0.1 ln(factor) + 1
-            (Peng et al., "YaRN: Efficient Context Window Extension of Large
-            Language Models", 2023, section 3).
+``yarn``    as bands, but mixed linearly in the pair's index, from the last whole
+            index at which a pair makes ``fast_turns`` (or 0) to the first at which it
+            makes ``slow_turns`` (at most rotary_dim - 1: the ramp may end beyond the
+            last of the rotary_dim / 2 pairs).  cos and sin are scaled by
+            0.1 ln(factor) + 1; a model with a factor of its own sets ``plan.gain``.
+
+Bands and the factor on cos and sin are those of Peng et al., "YaRN: Efficient Context
+Window Extension of Large Language Models", 2023, section 3; the ramp over the index is
+what models that name this method are trained with.
 
 The device form of f_i is f_i / 2 pi as a 64-bit binary fraction of a turn.
 """
@@ -65,7 +69,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
             return rotary_dim * math.log(original_len / (2 * math.pi * turns)) / (2 * math.log(base))
 
         first = max(math.floor(index(fast_turns)), 0)
-        last = min(math.ceil(index(slow_turns)), half - 1)
+        last = min(math.ceil(index(slow_turns)), rotary_dim - 1)
         keep = [1.0 - (i - first) / max(last - first, 1e-3) for i in range(half)]
         gain = 0.1 * math.log(factor) + 1.0
     keep = [min(1.0, max(0.0, k)) for k in keep]

@@ -1,9 +1,11 @@
 """What the decoder-layer operators and the model around them accept, refuse and
 promise, as far as that needs no GPU."""
 
+import math
+
 import pytest
 
-from qwen3_engine_from_scratch_b200.rope import RotaryPlan
+from qwen3_engine_from_scratch_b200.rope import RotaryPlan, rotary_frequencies
 
 TINY = dict(layers=1, hidden=32, heads=1, kv_heads=1, head_dim=16, intermediate=32, vocab=64, max_pos=8)
 
@@ -20,3 +22,28 @@ def test_model_refuses_plans_that_its_rotation_cannot_follow():
         Qwen3DecodeModel("cpu", rope_plan=RotaryPlan(18, device="cpu"), qk_norm=False, **TINY)
     whole = RotaryPlan(16, device="cpu")
     assert Qwen3DecodeModel("cpu", rope_plan=whole, **TINY).plan is whole
+
+
+def test_yarn_ramp_ends_beyond_the_last_pair_where_that_pair_still_turns():
+    """The ramp over the pair's index ends at the first whole index at which a pair
+    makes slow_turns or fewer, also where that lies past the last pair: written here
+    for one pair at a time, in turns."""
+    for rotary_dim, base, trained in ((128, 1e4, 131072), (64, 1e4, 131072), (128, 1e4, 65536), (26, 1e4, 32768),
+                                      (8, 1e4, 32768), (128, 1e6, 32768), (16, 1e6, 8192), (64, 5e5, 8192)):
+        factor, slow, fast = 4.0, 1.0, 32.0
+        turns = lambda i: trained * base ** (-2.0 * i / rotary_dim) / (2 * math.pi)  # noqa: E731
+        first, last = 0, 0
+        while turns(first + 1) >= fast:              # the last whole index with fast_turns or more
+            first += 1
+        while turns(last) > slow:                    # the first with slow_turns or fewer
+            last += 1
+        got, _ = rotary_frequencies(rotary_dim, base=base, scaling="yarn", factor=factor, original_len=trained,
+                                    slow_turns=slow, fast_turns=fast)
+        for i, f in enumerate(got):
+            squeezed = min(1.0, max(0.0, (i - first) / (last - first)))
+            plain = base ** (-2.0 * i / rotary_dim)
+            want = (1 - squeezed) * plain + squeezed * plain / factor
+            assert f == pytest.approx(want, rel=1e-12), (rotary_dim, base, trained, i)
+        # no pair that turns more than slow_turns is squeezed by the whole factor
+        assert all(f > 1.0001 * base ** (-2.0 * i / rotary_dim) / factor
+                   for i, f in enumerate(got) if turns(i) > slow)
