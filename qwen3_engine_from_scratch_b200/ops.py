@@ -952,6 +952,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out=None, residual_out=None):
     be ``residual`` itself.  (The reference's RMSNorm and addition:
     qwen3/norm.py:22-26; it rounds the sum to bf16 before the norm.)
     """
+    assert weight is not None, "weight must be (hidden,) bf16"
     return _norm(x, weight, residual, eps, False, out, residual_out, "b200_rms_norm")
 
 
@@ -962,6 +963,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, out=None, residual_out=None
     scale = max(max|y|, 1e-12) / 448 and q = e4m3(y / scale).  What ``linear``
     takes as ``x`` and ``x_scale``.
     """
+    assert weight is not None, "weight must be (hidden,) bf16"
     return _norm(x, weight, residual, eps, True, out, residual_out, "b200_rms_norm")
 
 

@@ -47,3 +47,13 @@ def test_yarn_ramp_ends_beyond_the_last_pair_where_that_pair_still_turns():
         # no pair that turns more than slow_turns is squeezed by the whole factor
         assert all(f > 1.0001 * base ** (-2.0 * i / rotary_dim) / factor
                    for i, f in enumerate(got) if turns(i) > slow)
+
+
+def test_norms_refuse_a_missing_weight():
+    """Not taken for a quantisation without a norm, which the C entry has for itself."""
+    import torch
+    from qwen3_engine_from_scratch_b200 import ops
+    x = torch.ones(2, 16, dtype=torch.bfloat16)
+    for norm in (ops.rms_norm, ops.rms_norm_fp8):
+        with pytest.raises(AssertionError, match="weight"):
+            norm(x, None)
