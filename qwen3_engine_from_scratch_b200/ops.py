@@ -1085,6 +1085,20 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     return y
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of t can lie at one place: in the order of the strides,
+    a dimension has to step past all that the ones before it span."""
+    if t.is_contiguous():
+        return False
+    span = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size > 1:
+            if stride < span:
+                return True
+            span += (size - 1) * stride
+    return False
+
+
 def _rotary_pair(t, out, dims, index, name):
     """q or k and its output, checked: contiguous heads, the same sizes."""
     assert t.dtype is _BF16 and t.dim() == dims and t.get_device() == index, \
@@ -1095,6 +1109,7 @@ def _rotary_pair(t, out, dims, index, name):
         return t, torch.empty_like(t, memory_format=torch.contiguous_format)
     assert out.shape == t.shape and out.dtype is _BF16 and out.stride(-1) == 1 and \
         out.get_device() == index, f"{name}_out must be like {name} with a contiguous head"
+    assert not _overlaps_itself(out), f"elements of {name}_out overlap"
     return t, out
 
 
@@ -1110,7 +1125,8 @@ def rotary(q, k, positions, plan, q_out=None, k_out=None):
     q: (T, H, D) with positions (T,), or (B, H, S, D) with positions (B, S);
     k: the same with its own number of heads, or None; bf16, any strides with a
     contiguous head.  The first ``plan.rotary_dim`` elements of every head turn, the
-    rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place).
+    rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place), and no
+    two elements of one may lie at one place.
     Any int32 or int64 position is exact to 2^-31 turns.
     """
     dims = q.dim()

@@ -57,3 +57,15 @@ def test_norms_refuse_a_missing_weight():
     for norm in (ops.rms_norm, ops.rms_norm_fp8):
         with pytest.raises(AssertionError, match="weight"):
             norm(x, None)
+
+
+def test_overlap_of_a_tensor_with_itself():
+    import torch
+    from qwen3_engine_from_scratch_b200 import ops
+    t = torch.zeros(4, 6, 16)
+    for fine in (t, t.transpose(0, 1), t[:, ::2], t[:, :, 3:9], t[:1].expand(1, 6, 16), t[:0], t[1:2, 3:4],
+                 t[0].unflatten(0, (2, 3)).transpose(0, 2), t.as_strided((1, 6, 16), (0, 16, 1))):
+        assert not ops._overlaps_itself(fine), (fine.shape, fine.stride())
+    for bad in (t[:1].expand(4, 6, 16), t[:, :1].expand(4, 6, 16), t.as_strided((4, 6, 16), (90, 16, 1)),
+                t.as_strided((4, 6, 16), (96, 15, 1)), t.as_strided((2, 4, 16), (24, 16, 1))):
+        assert ops._overlaps_itself(bad), (bad.shape, bad.stride())
