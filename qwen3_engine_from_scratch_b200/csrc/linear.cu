@@ -1069,7 +1069,9 @@ int linear_any(const void* x, int64_t x_stride, const float* x_scale, const void
                const void* residual, int64_t r_stride, void* out, int64_t o_stride,
                int m, int n, int k, int fp8, int gated, int activation,
                int32_t* dev_status, void* stream, bool any_address) {
-  if (m < 0 || n <= 0 || k <= 0 || n > 0x3fffffff || k > 0x1fffffff) return B200_ERR_INVALID_ARGUMENT;
+  // (2 n and the bytes of a row fit an int, and so does the last token tile's end)
+  if (m < 0 || n <= 0 || k <= 0 || m > 0x7fffffff - 255 || n > 0x3fffffff || k > 0x1fffffff)
+    return B200_ERR_INVALID_ARGUMENT;
   if (activation < B200_ACT_NONE || activation > B200_ACT_GELU_TANH)
     return B200_ERR_INVALID_ARGUMENT;
   if (m == 0) return B200_OK;

@@ -478,6 +478,9 @@ cudaError_t launch_wide(const NormArgs& a, dim3 grid, dim3 block, cudaStream_t c
   return b200host::launch_pdl(rms_norm_wide_kernel<VEC, true, false>, grid, block, 0, cs, a);
 }
 
+// a thread's element index steps past the row's end by a block's vectors at most
+constexpr int kMaxHidden = 0x7fffffff - 1024 * 8;
+
 bool multiple8(int64_t s) { return (s & 7) == 0; }
 bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -488,7 +491,8 @@ extern "C" int b200_rms_norm(const void* x, int64_t x_stride, const void* residu
                              float* scale, void* residual_out, int64_t h_stride, int64_t rows,
                              int hidden, float eps, int32_t* dev_status,
                              void* stream) {
-  if (rows < 0 || hidden <= 0 || rows > 0x7fffffff) return B200_ERR_INVALID_ARGUMENT;
+  if (rows < 0 || hidden <= 0 || hidden > kMaxHidden || rows > 0x7fffffff)
+    return B200_ERR_INVALID_ARGUMENT;
   if (rows == 0) return B200_OK;
   if (!x || !y || (residual == nullptr) != (residual_out == nullptr))
     return B200_ERR_INVALID_ARGUMENT;
@@ -527,19 +531,20 @@ extern "C" int b200_rms_norm(const void* x, int64_t x_stride, const void* residu
   // 48.0 us with 6 (66 held), 2000 x 12288 with norm and residual 29.8 with 2
   // (37.6 held), 8192 x 4096 39.6 with 8 (43.7 held).  Below the limits the held
   // form is as fast or faster (8192 x 1024: 11.7 us, streamed 14.1).
-  const int stage_bytes = (residual != nullptr ? 4 : 2) * hidden;
+  const int64_t stage_bytes = (residual != nullptr ? int64_t{4} : 2) * hidden;
   const int wide_from = weight != nullptr ? 2048 : 4096;
   if (vec && hidden >= wide_from && hidden <= 16384 &&
       rows >= static_cast<int64_t>(sms) * (weight != nullptr ? 2 : 4)) {
     int ctas = weight != nullptr ? (hidden <= 4096 ? 8 : hidden <= 6144 ? 4 : 2)
                                  : (hidden <= 4096 ? 8 : hidden <= 12288 ? 6 : 4);
     while (kStreamSmem / ctas < stage_bytes) ctas /= 2;
-    a.stages = kStreamSmem / ctas / stage_bytes;
+    a.stages = static_cast<int>(kStreamSmem / ctas / stage_bytes);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
     const int64_t most = static_cast<int64_t>(sms) * ctas;
     const int threads = ((hidden + 31) / 32 + 31) / 32 * 32;
     return b200host::status_from_cuda(launch_stream<4>(
-        a, static_cast<unsigned>(rows < most ? rows : most), threads, a.stages * stage_bytes, cs));
+        a, static_cast<unsigned>(rows < most ? rows : most), threads,
+        static_cast<int>(a.stages * stage_bytes), cs));
   }
   a.group = ((hidden + per - 1) / per + 31) / 32 * 32;
   cudaError_t e;

@@ -234,6 +234,8 @@ int plan_args(RotaryArgs& a, const void* positions, int64_t pos_stride_b, int64_
 
 constexpr int64_t kMaxBlocks = 0x7fffffff;
 constexpr int kMaxRotary = 8192;  // 32 KB of angles a token
+// a thread's head and slot indexes step past their ends by two blocks at most
+constexpr int kMaxHeads = 0x7fffffff - 1024, kMaxDim = kMaxHeads;
 
 }  // namespace
 
@@ -250,7 +252,9 @@ extern "C" int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h
   const int st = plan_args(a, positions, pos_stride_b, pos_stride_s, positions_64, turns, gain,
                            batch, seq, rotary_dim, interleaved);
   if (st != B200_OK) return st;
-  if (num_heads < 0 || num_kv_heads < 0 || head_dim < rotary_dim) return B200_ERR_INVALID_ARGUMENT;
+  if (num_heads < 0 || num_kv_heads < 0 || head_dim < rotary_dim || head_dim > kMaxDim ||
+      static_cast<int64_t>(num_heads) + num_kv_heads > kMaxHeads)
+    return B200_ERR_INVALID_ARGUMENT;
   a.heads = num_heads + num_kv_heads;
   if (a.tokens == 0 || a.heads == 0) return B200_OK;
   if (rotary_dim > kMaxRotary) return B200_ERR_UNSUPPORTED;

@@ -69,3 +69,23 @@ def test_overlap_of_a_tensor_with_itself():
     for bad in (t[:1].expand(4, 6, 16), t[:, :1].expand(4, 6, 16), t.as_strided((4, 6, 16), (90, 16, 1)),
                 t.as_strided((4, 6, 16), (96, 15, 1)), t.as_strided((2, 4, 16), (24, 16, 1))):
         assert ops._overlaps_itself(bad), (bad.shape, bad.stride())
+
+
+def test_c_entries_refuse_sizes_whose_indexes_would_pass_31_bits(native_lib):
+    """Element, token and head indexes are 32-bit and step past the end by a block's
+    share before the loops stop: sizes that close to 2^31 are refused, before a launch."""
+    lib, fake, top = native_lib, 16, 2 ** 31 - 1
+    norm = lambda hidden, weight: lib.b200_rms_norm(  # noqa: E731
+        fake, hidden, None, 0, weight, fake, hidden, None if weight else fake, None, 0, 1, hidden, 1e-6, None, None)
+    for hidden in (top, top - 7, top - 8191):
+        assert norm(hidden, fake) == -1 and norm(hidden, None) == -1, hidden
+    product = lambda m: lib.b200_linear(  # noqa: E731
+        fake, 8, None, fake, 8, None, None, None, 0, fake, 8, m, 8, 8, 0, 0, 0, None, None)
+    for m in (top, top - 1, top - 254):
+        assert product(m) == -1, m
+    rotary = lambda heads, kv, dim: lib.b200_rotary(  # noqa: E731
+        fake, 8, 8, 8, fake, 8, 8, 8, fake, 8, 8, 8, fake, 8, 8, 8, fake, 0, 1, 0, fake, 1.0, 1, 1, heads, kv, dim, 8,
+        0, None)
+    for heads, kv, dim in ((top, 1, 8), (top, 0, 8), (1, top - 512, 8), (2 ** 30, 2 ** 30, 8), (1, 1, top),
+                           (1, 1, top - 254)):
+        assert rotary(heads, kv, dim) == -1, (heads, kv, dim)
