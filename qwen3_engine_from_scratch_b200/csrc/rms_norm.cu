@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(512) rms_norm_stream_kernel(const NormArgs a) 
     bulk_load(dst, a.x + row * a.x_row, row_bytes, bar);
     if (a.r != nullptr) bulk_load(dst + row_bytes, a.r + row * a.r_row, row_bytes, bar);
   };
-  int issued = 0;
+  int issued = 0, taken = 0;  // copies (of thread 0), rows done; copy n is in stage n % stages
   if (t == 0) {
     for (int64_t row = blockIdx.x; issued < a.stages && row < a.rows; row += gridDim.x)
       fetch(row, issued++);
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(512) rms_norm_stream_kernel(const NormArgs a) 
   int s = 0;
   uint32_t phase = 0;
   int odd = 0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, odd ^= 1) {
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, odd ^= 1, ++taken) {
     bool ok = b200::mbar_wait_abortable(b200::smem_u32(&full[s]), phase, a.dev_status, kWaitLimitNs);
     const __nv_bfloat16* xr = reinterpret_cast<const __nv_bfloat16*>(ring + s * stage_bytes);
     float sum = 0.0f, top = 0.0f;
@@ -347,7 +347,10 @@ __global__ void __launch_bounds__(512) rms_norm_stream_kernel(const NormArgs a) 
     }
     if (t == 0) {
       const int64_t next = row + static_cast<int64_t>(a.stages) * gridDim.x;
-      if (next < a.rows) fetch(next, s);
+      if (next < a.rows) {
+        fetch(next, s);
+        ++issued;
+      }
     }
     float2 all = part[odd][0];
     for (int i = 1; i < warps; ++i) {
@@ -380,11 +383,11 @@ __global__ void __launch_bounds__(512) rms_norm_stream_kernel(const NormArgs a) 
     }
   }
   // after a give-up the copies in flight land before the shared memory goes away
-  if (t == 0 && a.dev_status != nullptr &&
-      (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT)) {
-    for (int i = 0; i < issued; ++i)
-      b200::mbar_wait_abortable(b200::smem_u32(&full[(s + i) % a.stages]),
-                                s + i < a.stages ? phase : phase ^ 1, nullptr, kWaitLimitNs / 10);
+  // (otherwise every copy was taken and there is none)
+  if (t == 0) {
+    for (; taken < issued; ++taken)
+      b200::mbar_wait_abortable(b200::smem_u32(&full[taken % a.stages]), (taken / a.stages) & 1,
+                                nullptr, kWaitLimitNs / 10);
   }
 }
 

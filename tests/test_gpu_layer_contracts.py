@@ -45,3 +45,37 @@ def test_rotary_refuses_outputs_whose_elements_overlap(qb):
     got, none = qb.rotary(src, None, p, plan, q_out=wide[:, 2:6])
     assert none is None and torch.equal(got, want)
     assert (wide[:, :2] == 0).all() and (wide[:, 6:] == 0).all()
+
+
+def _timed(call):
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    torch.cuda.synchronize()
+    begin.record()
+    out = call()
+    end.record()
+    torch.cuda.synchronize()
+    return out, begin.elapsed_time(end)
+
+
+def test_streamed_norm_does_not_wait_for_copies_that_nobody_issued(qb):
+    """Rows in numbers stream through shared memory.  Once its rows are done a block
+    has no copy under way, and a timeout that another kernel left on record must not
+    make it wait for one (0.1 s a stage)."""
+    x, w = _randn(_gen(2), 1000, 4096).to(BF16), torch.ones(4096, dtype=BF16, device="cuda")
+    qb.rms_norm(x, w)
+    qb.ops._status[torch.cuda.current_device()].fill_(0x10)       # B200_DEV_TIMEOUT
+    _, ms = _timed(lambda: qb.rms_norm(x, w))
+    qb.clear_device_status()
+    assert ms < 50, ms
+
+
+def test_streamed_norm_without_a_status_word(qb, native_lib):
+    """The C entry takes no status word too."""
+    x, r = _randn(_gen(3), 1000, 4096).to(BF16), _randn(_gen(4), 1000, 4096).to(BF16)
+    w = (1 + _randn(_gen(5), 4096, std=0.2)).to(BF16)
+    want, h = qb.rms_norm(x, w, residual=r)
+    y, h2 = torch.empty_like(x), torch.empty_like(x)
+    st = native_lib.b200_rms_norm(x.data_ptr(), 4096, r.data_ptr(), 4096, w.data_ptr(), y.data_ptr(), 4096, None,
+                                  h2.data_ptr(), 4096, 1000, 4096, 1e-6, None,
+                                  torch.cuda.current_stream().cuda_stream)
+    assert st == 0 and torch.equal(y, want) and torch.equal(h2, h)
