@@ -27,6 +27,12 @@ B200_DEVICE void flag_error(int32_t* dev_status, int32_t bits) {
   if (dev_status != nullptr) atomicOr(dev_status, bits);
 }
 
+// whether a kernel of this device gave up a wait since the host last cleared the status
+B200_DEVICE bool timeout_on_record(const int32_t* dev_status) {
+  return dev_status != nullptr &&
+         (*reinterpret_cast<const volatile int32_t*>(dev_status) & B200_DEV_TIMEOUT) != 0;
+}
+
 // ---------------------------------------------------------------- mbarrier
 B200_DEVICE void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

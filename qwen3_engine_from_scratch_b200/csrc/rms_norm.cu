@@ -271,12 +271,24 @@ __global__ void __launch_bounds__(512) rms_norm_stream_kernel(const NormArgs a) 
   const uint32_t row_bytes = static_cast<uint32_t>(a.hidden) * 2;
   const uint32_t stage_bytes = a.r != nullptr ? 2 * row_bytes : row_bytes;
   const int step = blockDim.x * 8;
+  // a pipeline gave up before this launch: no new work until the host clears the
+  // status.  Thread 0 reads it, so that the block agrees, and before the wait for the
+  // previous kernel, off the launch's path; once more after it where it is set, since
+  // that kernel may be the one that clears it.
+  __shared__ bool aborted;
   if (t == 0) {
     for (int s = 0; s < a.stages; ++s) b200::mbar_init(b200::smem_u32(&full[s]), 1);
     b200::fence_mbar_init();
+    aborted = b200::timeout_on_record(a.dev_status);
   }
   __syncthreads();
   b200::pdl_begin();
+  if (aborted) {
+    __syncthreads();
+    if (t == 0) aborted = b200::timeout_on_record(a.dev_status);
+    __syncthreads();
+    if (aborted) return;
+  }
   auto fetch = [&](int64_t row, int s) {
     const uint32_t bar = b200::smem_u32(&full[s]);
     const uint32_t dst = b200::smem_u32(ring) + s * stage_bytes;

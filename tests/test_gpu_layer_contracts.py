@@ -79,3 +79,23 @@ def test_streamed_norm_without_a_status_word(qb, native_lib):
                                   h2.data_ptr(), 4096, 1000, 4096, 1e-6, None,
                                   torch.cuda.current_stream().cuda_stream)
     assert st == 0 and torch.equal(y, want) and torch.equal(h2, h)
+
+
+def test_streamed_norm_waits_for_the_host_after_a_timeout(qb):
+    """With a timeout on record it starts nothing, as the other pipelined kernels: no
+    output is written in part.  Cleared, it works."""
+    x, r = _randn(_gen(6), 3000, 4096).to(BF16), _randn(_gen(7), 3000, 4096).to(BF16)
+    w = torch.ones(4096, dtype=BF16, device="cuda")
+    for norm, kind in ((qb.rms_norm, BF16), (qb.rms_norm_fp8, FP8)):
+        want = norm(x, w, residual=r)
+        out = torch.full((3000, 4096), 3.0, device="cuda").to(kind)
+        h = torch.full_like(r, 3.0)
+        qb.ops._status[torch.cuda.current_device()].fill_(0x10)       # B200_DEV_TIMEOUT
+        norm(x, w, residual=r, out=out, residual_out=h)
+        with pytest.raises(RuntimeError, match="timed out"):
+            qb.check_device_status()
+        assert (out.float() == 3.0).all() and (h == 3.0).all()
+        qb.clear_device_status()
+        got = norm(x, w, residual=r, out=out, residual_out=h)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+        qb.check_device_status()
