@@ -611,11 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const Tile first_tile = tile_at<BN, PAIR>(a, first, half);
   // a pipeline gave up before this launch: no new work until the host clears the
-  // status (read before the wait below: the load would be on every launch's path)
-  const bool aborted = a.dev_status != nullptr &&
-                       (*reinterpret_cast<const volatile int32_t*>(a.dev_status) & B200_DEV_TIMEOUT);
-  const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
-  if (warp == kWeightWarp && lane == 0 && first < tiles) {
+  // status (read before the wait below: the load would be on every launch's path; once
+  // more after it where it is set, since the previous kernel may be the one that clears it;
+  // the lanes of a warp agree: its waits are the whole warp's)
+  bool aborted = __any_sync(0xffffffffu, timeout_on_record(a.dev_status));
+  if (warp == kWeightWarp && lane == 0 && !aborted && first < a.m_tiles * a.n_tiles) {
     // The first weight tiles start towards L2 while the previous kernel drains (a
     // prefetch returns no data: what that kernel still writes is read after the wait).
     for (int p = kb0 * kPanels; p < min(kb1, kb0 + a.stages) * kPanels; ++p) {
@@ -625,6 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   pdl_begin();
+  if (aborted) aborted = __any_sync(0xffffffffu, timeout_on_record(a.dev_status));
+  const int tiles = aborted ? 0 : a.m_tiles * a.n_tiles;
 
   // The producer and MMA warps run their loops whole and one elected lane issues:
   // in a branch of a single lane every operand of a TMA or MMA instruction takes

@@ -99,3 +99,20 @@ def test_streamed_norm_waits_for_the_host_after_a_timeout(qb):
         got = norm(x, w, residual=r, out=out, residual_out=h)
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
         qb.check_device_status()
+
+
+def test_a_cleared_status_counts_from_the_next_call_on(qb):
+    """The clear is a kernel of its own, and the call behind it may be scheduled while
+    that one drains."""
+    x, w = _randn(_gen(8), 600, 4096).to(BF16), torch.ones(4096, dtype=BF16, device="cuda")
+    weight = _randn(_gen(9), 256, 4096, std=0.02).to(BF16)
+    status = qb.ops._status[torch.cuda.current_device()]
+    want_y, want_p = qb.rms_norm(x, w), qb.linear(x, weight)
+    for _ in range(50):
+        status.fill_(0x10)                                              # B200_DEV_TIMEOUT
+        status.zero_()
+        y = qb.rms_norm(x, w)
+        status.fill_(0x10)
+        status.zero_()
+        p = qb.linear(x, weight)
+        assert torch.equal(y, want_y) and torch.equal(p, want_p)
