@@ -160,7 +160,7 @@ B200_DEVICE void put_y(const NormArgs& a, int64_t row, int e, const float (&v)[V
 // norm (h has left by then), the row's own bf16 words without one (half the
 // registers, so twice the rows in flight: 8192 x 12288 in 103 us with fp32).
 template <int VEC, int NV, bool NORM, bool FP8>
-__global__ void __launch_bounds__(VEC == 8 && NV == 4 ? 512 : 1024) rms_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(VEC == 8 ? 512 : 1024) rms_norm_kernel(const NormArgs a) {
   b200::pdl_begin();
   __shared__ float2 part[32];
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.group) +
@@ -534,12 +534,15 @@ extern "C" int b200_rms_norm(const void* x, int64_t x_stride, const void* residu
                    (residual == nullptr ||
                     (multiple8(r_stride) && multiple8(h_stride) && aligned_to(residual, 16) &&
                      aligned_to(residual_out, 16)));
-  // A thread holds 4 vectors (or 8 single elements); few rows spread over more
-  // threads, one vector each, since their latency is all that counts.
+  // A thread holds 4 vectors (or 8 single elements); few rows of up to 4096 elements
+  // spread over more threads, one vector each, since their latency is all that counts.
+  // Beyond that 4 vectors are as fast or faster: in a graph, 1 x 8192 with residual to
+  // bf16 takes 2.4 us (3.0 with one vector and 1024 threads), 64 x 5120 to e4m3 2.35
+  // (2.44); 1 x 4104 to bf16 2.1 (2.0).
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int sms = b200host::sm_count(b200host::current_device());
   if (sms <= 0) return B200_ERR_CUDA;
-  const bool few = vec && hidden <= 8192 && rows <= sms;
+  const bool few = vec && hidden <= 4096 && rows <= sms;
   const int per = few ? 8 : vec ? 32 : 8;
   // Wide rows in numbers stream.  The CTAs an SM takes were swept from 1 to 8 for
   // rows of 1024 to 16384 elements: 8192 x 12288 to e4m3 without a norm takes

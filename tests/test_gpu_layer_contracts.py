@@ -116,3 +116,55 @@ def test_a_cleared_status_counts_from_the_next_call_on(qb):
         status.zero_()
         p = qb.linear(x, weight)
         assert torch.equal(y, want_y) and torch.equal(p, want_p)
+
+
+def _kernels(call):
+    """Names of the kernels that a call launches, from a graph of it."""
+    from cuda.bindings import driver
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        kept = call()                                       # noqa: F841
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    _, _, n = driver.cuGraphGetNodes(raw)
+    err, nodes, _ = driver.cuGraphGetNodes(raw, n)
+    assert err == driver.CUresult.CUDA_SUCCESS
+    names = []
+    for node in nodes:
+        err, kind = driver.cuGraphNodeGetType(node)
+        if err == driver.CUresult.CUDA_SUCCESS and kind == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            err, p = driver.cuGraphKernelNodeGetParams(node)
+            assert err == driver.CUresult.CUDA_SUCCESS
+            err, name = driver.cuKernelGetName(p.kern) if int(p.func) == 0 else driver.cuFuncGetName(p.func)
+            assert err == driver.CUresult.CUDA_SUCCESS
+            names.append(name.decode())
+    return names
+
+
+@pytest.mark.parametrize("rows,hidden", [(1, 4096), (1, 4104), (8, 5120), (3, 6144), (64, 8192), (148, 8192),
+                                         (2, 8200), (5, 16384)])
+def test_few_wide_rows_are_read_once(qb, rows, hidden):
+    """A decode step's rows stay in registers up to 16,384 elements: no second read."""
+    from test_gpu_layer_ops import _check_bf16, _check_fp8, _norm_exact
+    g = _gen(rows * hidden)
+    x, r = _randn(g, rows, hidden, std=2.0).to(BF16), _randn(g, rows, hidden, std=3.0).to(BF16)
+    w = (1 + _randn(g, hidden, std=0.3)).to(BF16)
+    for res in (None, r):
+        want, h = _norm_exact(x, w, res, 1e-6)
+        got, q = qb.rms_norm(x, w, residual=res), qb.rms_norm_fp8(x, w, residual=res)
+        _check_bf16(got if res is None else got[0], want)
+        _check_fp8(q[0], q[1], want)
+        if res is not None:
+            _check_bf16(got[1], h)
+            assert torch.equal(got[1], q[2])
+    _check_fp8(*qb.quantize_rows_fp8(x), x.double())
+    for call in (lambda: qb.rms_norm(x, w, residual=r), lambda: qb.rms_norm_fp8(x, w),
+                 lambda: qb.quantize_rows_fp8(x)):
+        names = _kernels(call)
+        assert len(names) == 1 and "rms_norm_kernel" in names[0], names
+
+
+def test_wider_rows_are_read_twice(qb):
+    x, w = torch.ones(2, 16392, dtype=BF16, device="cuda"), torch.ones(16392, dtype=BF16, device="cuda")
+    names = _kernels(lambda: qb.rms_norm(x, w))
+    assert len(names) == 1 and "rms_norm_wide_kernel" in names[0], names
