@@ -40,9 +40,8 @@
 //
 // Every wait is bounded: one that runs out sets B200_DEV_TIMEOUT, the other
 // roles give up too, outstanding copies are awaited and TMEM is freed.
-#include <mutex>
-
 #include "linear.cuh"
+#include "once.cuh"
 #include "tcgen05.cuh"
 #include "words.cuh"
 
@@ -818,11 +817,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ host side
 
-std::mutex g_attr_mu;
-bool g_attr_done[64] = {false};
+b200host::OncePerDevice g_setup;
 // CTAs of clusters of 1, 2, 4 and 8 that a device holds at once (clusters do not
 // span its GPCs: 8 CTAs a cluster leave some SMs without one)
-int g_resident[64][4];
+int g_resident[b200host::OncePerDevice::kDevices][4];
 
 template <int BN, bool FP8, bool PAIR>
 cudaError_t set_smem_attr() {
@@ -840,11 +838,7 @@ cudaError_t set_smem_attrs() {
   return cudaSuccess;
 }
 
-int ensure_smem_attr(int dev) {
-  if (dev < 0 || dev >= 64) return B200_ERR_CUDA;
-  if (g_attr_done[dev]) return B200_OK;
-  std::lock_guard<std::mutex> lk(g_attr_mu);
-  if (g_attr_done[dev]) return B200_OK;
+int set_up(int dev) {
   cudaError_t e = set_smem_attrs<false>();
   if (e == cudaSuccess) e = set_smem_attrs<true>();
   if (e != cudaSuccess) return b200host::status_from_cuda(e);
@@ -866,8 +860,12 @@ int ensure_smem_attr(int dev) {
     if (e != cudaSuccess) return b200host::status_from_cuda(e);
     g_resident[dev][i] = clusters << i;
   }
-  g_attr_done[dev] = true;
   return B200_OK;
+}
+
+int ensure_set_up(int dev) {
+  if (dev < 0 || dev >= b200host::OncePerDevice::kDevices) return B200_ERR_CUDA;
+  return g_setup.run(dev, [dev] { return set_up(dev); });
 }
 
 // How a product is cut: token tiles of bn, 128 weight rows a CTA or 256 a pair of
@@ -1110,7 +1108,7 @@ int linear_any(const void* x, int64_t x_stride, const float* x_scale, const void
   if (b200host::linear_is_small(a, k, fp8 != 0))
     return b200host::status_from_cuda(
         b200host::linear_small(a, x, x_stride, w, w_stride, k, fp8 != 0, sms, cs));
-  int st = ensure_smem_attr(dev);
+  int st = ensure_set_up(dev);
   if (st != B200_OK) return st;
 
   const int tile_n = gated ? kRows / 2 : kRows;

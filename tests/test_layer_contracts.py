@@ -2,9 +2,13 @@
 promise, as far as that needs no GPU."""
 
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 
+from qwen3_engine_from_scratch_b200 import rope
 from qwen3_engine_from_scratch_b200.rope import RotaryPlan, rotary_frequencies
 
 TINY = dict(layers=1, hidden=32, heads=1, kv_heads=1, head_dim=16, intermediate=32, vocab=64, max_pos=8)
@@ -89,3 +93,60 @@ def test_c_entries_refuse_sizes_whose_indexes_would_pass_31_bits(native_lib):
     for heads, kv, dim in ((top, 1, 8), (top, 0, 8), (1, top - 512, 8), (2 ** 30, 2 ** 30, 8), (1, 1, top),
                            (1, 1, top - 254)):
         assert rotary(heads, kv, dim) == -1, (heads, kv, dim)
+
+
+ONCE = r"""
+#include <cstdio>
+#include <thread>
+#include <vector>
+#include "once.cuh"
+
+static b200host::OncePerDevice once;
+static int calls[64], value[64][4];   // plain data behind the flag, as the products' occupancies
+
+int main() {
+  int failures = 0;
+  if (once.run(3, [] { return -5; }) != -5) ++failures;      // a failure is not kept
+  for (int device = 0; device < 64; ++device) {
+    std::vector<std::thread> threads;
+    std::vector<int> seen(8);
+    for (int t = 0; t < 8; ++t)
+      threads.emplace_back([&, t] {
+        if (once.run(device, [&] { ++calls[device]; for (int& v : value[device]) v = device + 1; return 0; }) == 0)
+          seen[t] = value[device][t % 4];
+      });
+    for (auto& t : threads) t.join();
+    for (int v : seen) failures += v != device + 1;
+    failures += calls[device] != 1;
+  }
+  return failures != 0;
+}
+"""
+
+
+def test_first_calls_from_several_threads(tmp_path):
+    """One thread does a device's first-call work, the others see all of it; under the
+    thread sanitizer, which exits with 66 where it finds a race."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    csrc = os.path.join(os.path.dirname(rope.__file__), "csrc")
+
+    def run(source):
+        (tmp_path / "t.cc").write_text(source)
+        exe = str(tmp_path / "t")
+        built = subprocess.run([gxx, "-std=c++17", "-O1", "-g", "-fsanitize=thread", "-I", csrc,
+                                str(tmp_path / "t.cc"), "-o", exe], capture_output=True, text=True)
+        if built.returncode:
+            return None, built.stderr
+        done = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+        return done.returncode, done.stderr
+
+    if run("int main() { return 0; }")[0] != 0:
+        pytest.skip("the thread sanitizer does not run here")
+    code, text = run(ONCE)
+    assert code == 0, text[-3000:]
+    # linear.cu keeps its occupancies behind it, and no flag of its own
+    with open(os.path.join(csrc, "linear.cu")) as f:
+        source = f.read()
+    assert "OncePerDevice" in source and "g_attr_done" not in source
