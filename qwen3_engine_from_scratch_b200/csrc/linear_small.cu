@@ -196,11 +196,9 @@ cudaError_t linear_small(const b200::LinearArgs& e, const void* x, int64_t x_str
   // them: 8 x 4096 x 2048 6.3 -> 5.5 us, 1 x 2048 x 1024 3.2 -> 2.5; with two blocks an
   // SM 8 warps are faster (8 x 4096 x 4096 8.5, 10.3 with 16).
   const bool wide = blocks <= static_cast<unsigned>(sms) && a.k_bytes >= 8 * 8 * kStep;
-  if (!aligned) {
-    if (e.m > 8) return launch<2, 2, 8, false>(a, fp8, blocks, stream);
+  if (!aligned)  // at most 8 tokens: b200_linear_unaligned takes no more
     return wide ? launch<1, 2, 16, false>(a, fp8, blocks, stream)
                 : launch<1, 2, 8, false>(a, fp8, blocks, stream);
-  }
   if (e.m > 8) return launch<2, 4, 8, true>(a, fp8, blocks, stream);
   if (wide) return launch<1, 4, 16, true>(a, fp8, blocks, stream);
   // Eight steps ahead with up to two blocks an SM: 8 x 12288 x 4096 23.3 -> 20.7; with
