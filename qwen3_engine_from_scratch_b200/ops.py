@@ -1009,8 +1009,8 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     ``gated``: weight holds n gate rows, then n up rows (bias and weight_scale
     too), and the result is act(gate) * up + residual.  ``activation``: None, "relu",
     "silu", "gelu" (error function) or "gelu_tanh".  bias: bf16; residual and
-    ``out``: (..., n) bf16, ``out`` may be ``residual``.  Everything between the
-    operands and the one rounding at the end is fp32.  Above 8 tokens, operands
+    ``out``: (..., n) bf16, ``out`` may be ``residual`` and overlaps nothing else.
+    Everything between the operands and the one rounding at the end is fp32.  Above 8 tokens, operands
     whose rows do not lie on 16-byte boundaries are copied to padded rows first.
     """
     assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
@@ -1062,6 +1062,8 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
         y_stride = n
     else:
         y, y_stride = out, max(n, _out_rows(out, shape, _BF16, index, "out").stride(0))
+        assert out.data_ptr() not in (x.data_ptr(), weight.data_ptr()) or out.numel() == 0, \
+            "out overlaps an operand"
     any_address = False
     unit = 16 if fp8 else 8
     if k % unit == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:

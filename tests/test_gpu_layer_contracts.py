@@ -168,3 +168,17 @@ def test_wider_rows_are_read_twice(qb):
     x, w = torch.ones(2, 16392, dtype=BF16, device="cuda"), torch.ones(16392, dtype=BF16, device="cuda")
     names = _kernels(lambda: qb.rms_norm(x, w))
     assert len(names) == 1 and "rms_norm_wide_kernel" in names[0], names
+
+
+def test_product_refuses_its_operand_as_its_output(qb):
+    """Other blocks still read x and the weight when a block writes its outputs."""
+    x = _randn(_gen(10), 64, 64).to(BF16)
+    w = _randn(_gen(11), 64, 64, std=0.1).to(BF16)
+    for bad in (x, w):
+        with pytest.raises(AssertionError, match="overlap"):
+            qb.linear(x, w, out=bad)
+    wide = torch.zeros(64, 128, dtype=BF16, device="cuda")          # side by side in one tensor
+    wide[:, :64] = x
+    qb.linear(wide[:, :64], w, out=wide[:, 64:])
+    assert torch.equal(wide[:, 64:], qb.linear(x, w)) and torch.equal(wide[:, :64], x)
+    assert qb.linear(x[:0], w, out=x[:0]).shape == (0, 64)
