@@ -1010,8 +1010,9 @@ def linear(x, weight, bias=None, activation=None, gated=False, residual=None, ou
     too), and the result is act(gate) * up + residual.  ``activation``: None, "relu",
     "silu", "gelu" (error function) or "gelu_tanh".  bias: bf16; residual and
     ``out``: (..., n) bf16, ``out`` may be ``residual`` and overlaps nothing else.
-    Everything between the operands and the one rounding at the end is fp32.  Above 8 tokens, operands
-    whose rows do not lie on 16-byte boundaries are copied to padded rows first.
+    Everything between the operands and the one rounding at the end is fp32.  Above 8
+    tokens, operands whose rows do not lie on 16-byte boundaries are copied to padded
+    rows first.
     """
     assert activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)}"
     dtype = x.dtype
