@@ -5,10 +5,11 @@
 // interleaved one; the rest of the head is copied.
 //
 // Angles: the plan holds f_i / 2 pi as a 64-bit binary fraction of a turn, so
-// position * f_i modulo one turn is one 64-bit integer product, exact to
-// position * 2^-64 turns at any position (negative ones included); the top 32
-// bits then go through sincospi.  A product in fp32 would lose position * 2^-24
-// radians: 0.008 at position 131,072.
+// position * f_i modulo one turn is one 64-bit integer product, at any position
+// (negative ones included).  Its top 32 bits, rounded to fp32 (2^-26 turns near half a
+// turn), go through sincospi.  The fractions come from float64 frequencies and are off
+// by up to 2^-54 turns a position, less than that rounding up to position 2^28.  A
+// product in fp32 would lose position * 2^-24 radians: 0.008 at position 131,072.
 //
 // Bound by memory for prefills: q and k are read and written once.  A block
 // takes a few tokens: it computes their sines and cosines once into shared

@@ -1130,7 +1130,8 @@ def rotary(q, k, positions, plan, q_out=None, k_out=None):
     contiguous head.  The first ``plan.rotary_dim`` elements of every head turn, the
     rest is copied.  ``q_out`` / ``k_out`` may be q and k themselves (in place), and no
     two elements of one may lie at one place.
-    Any int32 or int64 position is exact to 2^-31 turns.
+    Positions are any int32 or int64 values; an angle is off by at most 2^-26 turns (its
+    rounding to fp32) and |position| 2^-54 turns (the plan's float64 frequencies).
     """
     dims = q.dim()
     assert dims in (3, 4), "q must be (T, heads, D) or (B, heads, S, D)"

@@ -22,7 +22,8 @@ Bands and the factor on cos and sin are those of Peng et al., "YaRN: Efficient C
 Window Extension of Large Language Models", 2023, section 3; the ramp over the index is
 what models that name this method are trained with.
 
-The device form of f_i is f_i / 2 pi as a 64-bit binary fraction of a turn.
+The device form of f_i is f_i / 2 pi as a 64-bit binary fraction of a turn, from the
+float64 f_i: off by up to 2^-54 turns a position.
 """
 
 from __future__ import annotations
@@ -91,6 +92,7 @@ class RotaryPlan:
                                                   original_len, slow_turns, fast_turns)
         self.turns = torch.tensor([_signed64(round(f / (2 * math.pi) * 2.0 ** 64)) for f in self.freq],
                                   dtype=torch.int64, device=device)
+
 
 def _signed64(v):
     v &= (1 << 64) - 1

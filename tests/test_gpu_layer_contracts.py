@@ -182,3 +182,27 @@ def test_product_refuses_its_operand_as_its_output(qb):
     qb.linear(wide[:, :64], w, out=wide[:, 64:])
     assert torch.equal(wide[:, 64:], qb.linear(x, w)) and torch.equal(wide[:, :64], x)
     assert qb.linear(x[:0], w, out=x[:0]).shape == (0, 64)
+
+
+@pytest.mark.parametrize("rotary_dim,base", [(128, 1000000), (64, 10000)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_angles_at_any_position(qb, rotary_dim, base, layout):
+    """An angle is off by 2^-26 turns (32 bits of a turn rounded to fp32: 2^-26, and cut
+    there: 2^-32) and 2^-54 turns a position (the plan's frequencies); sine and cosine
+    by 2^-22 more."""
+    import math
+    from decimal import Decimal, localcontext
+    from test_layer_contracts import turns_a_position
+    at = [0, 1, -1, 17, 131071, -4097, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31, 2 ** 33 + 5, -(2 ** 37) + 3, 2 ** 40 + 9]
+    plan = qb.RotaryPlan(rotary_dim, base=float(base), layout=layout)
+    cos, sin = (t.double().cpu() for t in qb.rotary_tables(torch.tensor(at, device="cuda"), plan))
+    exact = turns_a_position(rotary_dim, base)
+    for row, p in enumerate(at):
+        bound = 2 * math.pi * (2.0 ** -26 + 2.0 ** -32 + abs(p) * 2.0 ** -54) + 2.0 ** -22
+        for i, f in enumerate(exact):
+            with localcontext() as c:
+                c.prec = 60
+                part = float((f * p) % 1)
+            for e in ((i, i + rotary_dim // 2) if layout == "half" else (2 * i, 2 * i + 1)):
+                assert abs(float(cos[row, e]) - math.cos(2 * math.pi * part)) <= bound, (p, i)
+                assert abs(float(sin[row, e]) - math.sin(2 * math.pi * part)) <= bound, (p, i)

@@ -5,6 +5,7 @@ import math
 import os
 import shutil
 import subprocess
+from decimal import Decimal, localcontext
 
 import pytest
 
@@ -150,3 +151,28 @@ def test_first_calls_from_several_threads(tmp_path):
     with open(os.path.join(csrc, "linear.cu")) as f:
         source = f.read()
     assert "OncePerDevice" in source and "g_attr_done" not in source
+
+
+PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803")
+
+
+def turns_a_position(rotary_dim, base, factor=1):
+    """rotary_dim / 2 exact turns a position (to 50 digits), f_i / factor."""
+    with localcontext() as c:
+        c.prec = 60
+        return [(Decimal(base) ** (Decimal(-2 * i) / rotary_dim)) / factor / (2 * PI) for i in range(rotary_dim // 2)]
+
+
+@pytest.mark.parametrize("rotary_dim,base", [(128, 1000000), (64, 10000), (6, 100), (256, 500000)])
+def test_fractions_of_a_turn_against_50_digits(rotary_dim, base):
+    """The plan's float64 frequencies leave 2^-54 of a turn a position: pow's and the
+    exponent's rounding, 1.4 x 2^-53 of f <= 1, and 2 pi's and the quotient's, 1.4 more,
+    all over 2 pi."""
+    for factor in (1, 4):
+        more = dict(scaling="linear", factor=float(factor)) if factor > 1 else {}
+        plan = RotaryPlan(rotary_dim, base=float(base), device="cpu", **more)
+        for got, want in zip(plan.turns.tolist(), turns_a_position(rotary_dim, base, factor)):
+            with localcontext() as c:
+                c.prec = 60
+                off = abs(Decimal(got % 2 ** 64) / 2 ** 64 - want)
+            assert off < Decimal(2) ** -54
