@@ -71,8 +71,9 @@ const char* b200_last_cuda_error_string(void);
  * holds B200_DEV_TIMEOUT (how one timed-out CTA ends the rest of its grid),
  * then ORs B200_DEV_TIMEOUT into *dev_status and writes 0 to *result (1 if the
  * wait had completed).  The kernel returns normally: the CUDA context stays
- * usable, and kernels that check the status word (the prefill) start no new
- * work until the caller clears it. */
+ * usable, and kernels that check the status word (the prefill, the pipelined
+ * product, the norm of many wide rows) start no new work until the caller
+ * clears it. */
 int b200_selftest_bounded_wait(int32_t* dev_status, int32_t* result, uint64_t limit_ns,
                                void* stream);
 
@@ -399,7 +400,7 @@ int b200_qk_norm_rope_kv_write(
  * or not at all.  weight == NULL: no norm, y = x (needs scale, no residual).
  * Row strides in elements; rows contiguous; x, residual, weight, residual_out
  * bf16.  residual_out may be residual or x.  Rows that are 16-byte aligned
- * take the vector path, others any alignment.
+ * take the vector path, others any alignment.  At most 2^31 - 8193 elements a row.
  */
 int b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
                   const void* weight, void* y, int64_t y_stride, float* scale,
@@ -423,7 +424,7 @@ int b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t
  * NULL where unused.  Row strides in elements, rows contiguous; x and w start on
  * 16 bytes and their row strides are multiples of 16 bytes (k itself need not
  * be); out may be residual, and overlaps nothing else.  Sums in fp32, one
- * rounding.
+ * rounding.  m at most 2^31 - 256, n 2^30 - 1, k 2^29 - 1.
  */
 int b200_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w,
                 int64_t w_stride, const float* w_scale, const void* bias, const void* residual,
@@ -449,7 +450,8 @@ int b200_pack_rows(const void* src, int64_t src_stride, void* dst, int64_t dst_s
  * (pairs i, i + rotary_dim / 2, or 2i, 2i + 1 when interleaved), the rest is
  * copied.  turns: rotary_dim / 2 fractions of a turn a position, in units of
  * 2^-64; gain multiplies cos and sin.  positions: int32 or int64 (batch, seq)
- * with strides.  num_heads or num_kv_heads may be 0.
+ * with strides.  num_heads or num_kv_heads may be 0; rotary_dim is at most 8192,
+ * and no two elements of an output lie at one place.
  * (The reference turns by tables, qwen3/rope.py:88-110.)
  */
 int b200_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,

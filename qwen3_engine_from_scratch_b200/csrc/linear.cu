@@ -30,11 +30,11 @@
 // order, so the result does not depend on timing.  Up to 8 tokens (16 with a small
 // weight) go to the direct kernel of linear_small.cu.
 //
-// Bounds and what it measured (B200): large products by the tensor pipe, 95 %
-// active in bf16 and 91 % in e4m3 at the 1.5 GHz that the power cap leaves: 4096
-// tokens, 4096 -> 2 x 12288 gated with silu in 584 us (1.41 PFLOP/s) and 319 us
-// (2.59 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
-// of tiles: 90 us (4.3 TB/s; 81 into one output that partly stays in L2).  64 x 12288 x
+// Bounds and what it measured (B200): large products by the tensor pipe, 97 %
+// active in bf16 and 95 % in e4m3 at the 1.5 GHz that the power cap leaves: 4096
+// tokens, 4096 -> 2 x 12288 gated with silu in 586 us (1.41 PFLOP/s) and 320 us
+// (2.58 PFLOP/s).  256 rows of 151,936 logits by the memory and the last of 9 rounds
+// of tiles: 89 us (4.4 TB/s; 81 into one output that partly stays in L2).  64 x 12288 x
 // 4096 in e4m3 by the weight's bytes and about 5 us of launch, first loads, exchange
 // and end: 12.8 us (4.0 TB/s), 13.7 with a residual.
 //

@@ -19,8 +19,8 @@
 // the shuffles together.  Sums, maxima and scales are fp32; NaN propagates into
 // the scale (max.NaN), so a row that holds one is NaN throughout, as its
 // definition says.
-// Measured: 8192 x 4096 with residual to e4m3 40.9 us (5.8 TB/s, 0.88 of the copy
-// rate), to bf16 44 us (0.93); 8192 x 12288 to e4m3 without a norm 49.7 us (0.93); one
+// Measured: 8192 x 4096 with residual to e4m3 40.5 us (5.8 TB/s, 0.88 of the copy
+// rate), to bf16 44 us (0.93); 8192 x 12288 to e4m3 without a norm 49.2 us (0.93); one
 // row of 1024 1.5 us in a graph, its latency.
 #include "common.cuh"
 #include "words.cuh"
